@@ -357,6 +357,90 @@ typedef struct {
 
 int g3k_gemm(const g3k_gemm_args *a, void *stream);
 
+/* ---- KV cache in pages (pages.hip, paged_attn.hip) ----
+ * Pages: [page][n_kv_heads][page size][D], fp32 or bf16, pages page_stride
+ * elements apart; page size = 1 << page_shift (16 .. 1024).  A sequence's
+ * positions are its table row's pages in order.  Lengths, tables, row offsets
+ * and group bounds are device arrays that the kernels keep within their
+ * buffers: a length is cut to its table, a page outside the pool is not
+ * followed.  At most G3K_PAGED_MAX_SEQS sequences and G3K_PAGED_MAX_LEN
+ * positions each. */
+#define G3K_PAGED_MAX_SEQS 4096
+#define G3K_PAGED_MAX_LEN (1 << 24)
+typedef struct {
+    const int *kv_len;       /* [num_seqs] keys, new tokens included */
+    const int *page_table;   /* [num_seqs][table_stride] */
+    const int *q_start;      /* [num_seqs + 1] first packed row, or NULL: one row a sequence */
+    int num_seqs, table_stride, total_q, page_shift;
+} g3k_paged_seqs;
+
+/* QK-norm + RoPE of total_q packed tokens (the last of their sequences): q to
+ * q_out [total_q][heads][D], k and v to their pages.  Rows that no sequence
+ * has, and positions outside [0, max_context), are left alone. */
+typedef struct {
+    g3k_paged_seqs s;
+    const float *Q, *K, *V;
+    const uint16_t *q_norm, *k_norm;   /* both or none */
+    const float *rope;
+    float eps;
+    float *q_out;
+    void *k, *v;
+    int bf16, num_pages, n_kv_heads, group, max_context;
+    long long page_stride;
+} g3k_paged_write_args;
+int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
+
+/* Attention of packed tokens (prefill) or of one token per sequence (decode)
+ * over pages; q and out [total_q][heads][D].  blocks: 16-row blocks per wave
+ * (1 or 2: 64 or 128 rows per workgroup).
+ * Prefill: items bounds the row blocks of the batch, sum over sequences of
+ * ceil(tokens * group / (64 blocks)); each block's keys go to up to `parts`
+ * workgroups, whose parts [items][parts][n_kv_heads][64 blocks] rows a second
+ * launch joins.
+ * Decode: group i's members [group_start[i], group_start[i + 1]) share their
+ * first prefix_len[i] positions, read once through the first member's table.
+ * The keys are cut into about `budget` chunks per KV head, at most `items`,
+ * of at least min_tiles 32-key tiles; parts [items][n_kv_heads][part_rows]
+ * rows, found through the directories dir_prefix and dir_tail [num_seqs][2]. */
+typedef struct {
+    g3k_paged_seqs s;
+    const void *k, *v;
+    int bf16, num_pages, n_kv_heads, group, window;
+    long long page_stride;
+    float qscale;              /* softmax scale * log2(e) */
+    const float *q;
+    float *out;
+    int blocks, items, parts;
+    float *part_o, *part_ml;   /* D floats, and (max, sum), per row */
+    int n_groups;
+    const int *group_start, *prefix_len;
+    int budget, min_tiles, part_rows;
+    int *dir_prefix, *dir_tail;
+} g3k_paged_args;
+int g3k_paged_prefill(const g3k_paged_args *a, void *stream);
+int g3k_paged_decode(const g3k_paged_args *a, void *stream);
+
+/* Forks and compaction of the sequences in a pool of num_layers layers'
+ * pages, each layer's pages layer_stride elements after the last one's.
+ * elem: bytes per element.  Scratch: ref, writers, first, list, list2, map
+ * [num_pages], rows [n_out][table_stride], child [n_out], count [1]. */
+typedef struct {
+    int old_len, want, kept, full, tail, offset, granted, copy;
+} g3k_fork_child;
+typedef struct {
+    void *k, *v;
+    int elem, num_layers, num_pages, page_shift, n_kv_heads, table_stride;
+    long long page_stride, layer_stride;
+    int n_in, n_out;
+    const int *len_in, *table_in, *parent, *add, *held;
+    int *len_out, *table_out, *status;
+    int *ref, *writers, *first, *list, *list2, *map, *rows, *count;
+    g3k_fork_child *child;
+    int copy_wgs;              /* compaction: workgroups that copy */
+} g3k_pages_args;
+int g3k_pages_fork(const g3k_pages_args *a, void *stream);
+int g3k_pages_compact(const g3k_pages_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

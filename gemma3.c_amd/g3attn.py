@@ -113,6 +113,11 @@ def lib():
     L.g3attn_matmul_bf16_device.argtypes = [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int]
     L.g3attn_forward_token_device.argtypes = [_vp, C.c_int, C.c_int, _vp]
     L.g3attn_prefill_forward_device.argtypes = [_vp, C.c_void_p, _i32p, C.c_int, C.c_int, _vp]
+    L.g3attn_paged_write_device.argtypes = [_vp, C.c_int] + [_vp] * 8
+    L.g3attn_paged_prefill_device.argtypes = [_vp, C.c_int] + [_vp] * 4
+    L.g3attn_paged_decode_device.argtypes = [_vp, C.c_int] + [_vp] * 5
+    L.g3attn_pages_fork_device.argtypes = [_vp] * 8
+    L.g3attn_pages_compact_device.argtypes = [_vp] * 6
     for name in ("g3attn_decode", "g3attn_prefill", "g3attn_decode_device",
                  "g3attn_prefill_device", "g3attn_kv_append", "g3attn_kv_append_device",
                  "g3attn_kv_write", "g3attn_kv_read", "g3attn_synchronize",
@@ -121,7 +126,9 @@ def lib():
                  "g3attn_forward_device", "g3attn_upload_weights", "g3attn_forward_token",
                  "g3attn_prefill_tokens", "g3attn_matmul_bf16_device",
                  "g3attn_prefill_forward_device", "g3attn_forward_token_device",
-                 "g3attn_gqa_noalloc", "g3attn_upload_rope", "g3attn_last_splits"):
+                 "g3attn_gqa_noalloc", "g3attn_upload_rope", "g3attn_last_splits",
+                 "g3attn_paged_write_device", "g3attn_paged_prefill_device", "g3attn_paged_decode_device",
+                 "g3attn_pages_fork_device", "g3attn_pages_compact_device"):
         getattr(L, name).restype = C.c_int
     _lib = L
     return L
@@ -235,6 +242,35 @@ def host_weights(embed: np.ndarray, layers, norm: np.ndarray):
         for name in LAYER_TENSORS:
             setattr(W.layers[l], name, ptr(lw.get(name)))
     return W, keep
+
+
+PAGE_F32, PAGE_BF16 = 0, 1   # G3ATTN_PAGE_*
+
+
+class Pages(C.Structure):
+    """g3attn_pages: a pool of pages for layers first_layer.. (device addresses)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("first_layer", C.c_int),
+                ("num_layers", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int),
+                ("page_stride", C.c_longlong), ("layer_stride", C.c_longlong)]
+
+
+class Seqs(C.Structure):
+    """g3attn_seqs: lengths and page tables of sequences (device addresses)."""
+    _fields_ = [("num_seqs", C.c_int), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int)]
+
+
+class Batch(C.Structure):
+    """g3attn_batch: packed new tokens of sequences; q_start None: one each."""
+    _fields_ = [("seqs", Seqs), ("total_q", C.c_int), ("q_start", C.c_void_p)]
+
+
+class Prefixes(C.Structure):
+    """g3attn_prefixes: runs of sequences that share their first positions."""
+    _fields_ = [("num_groups", C.c_int), ("group_start", C.c_void_p), ("prefix_len", C.c_void_p)]
+
+
+def _ref(s):
+    return None if s is None else C.byref(s)
 
 
 class Context:
@@ -435,3 +471,25 @@ class Context:
         v = np.empty((n, self.ks), dtype=np.float32)
         _check(lib().g3attn_kv_read(self._h, layer, slot, n, k, v))
         return k, v
+
+    # ---- KV cache in pages: device addresses, enqueued on the context's stream
+
+    def paged_write_device(self, layer, pages: Pages, batch: Batch, Q, K, V, q_norm, k_norm, q_out):
+        """QK-norm + RoPE of packed tokens: q to q_out, K and V to their pages."""
+        _check(lib().g3attn_paged_write_device(self._h, layer, _ref(pages), _ref(batch), Q, K, V, q_norm, k_norm, q_out))
+
+    def paged_prefill_device(self, layer, pages: Pages, batch: Batch, q, out):
+        """Causal attention of packed tokens over their sequences' pages."""
+        _check(lib().g3attn_paged_prefill_device(self._h, layer, _ref(pages), _ref(batch), q, out))
+
+    def paged_decode_device(self, layer, pages: Pages, batch: Batch, prefixes: "Prefixes | None", q, out):
+        """Attention of one token per sequence; shared prefixes are read once."""
+        _check(lib().g3attn_paged_decode_device(self._h, layer, _ref(pages), _ref(batch), _ref(prefixes), q, out))
+
+    def pages_fork_device(self, pages: Pages, src: Seqs, parent, add, held, dst: Seqs, status=None):
+        """Sequences dst from src: forked, grown or cut by add, ended."""
+        _check(lib().g3attn_pages_fork_device(self._h, _ref(pages), _ref(src), parent, add, held, _ref(dst), status))
+
+    def pages_compact_device(self, pages: Pages, src: Seqs, held, dst: Seqs, status=None):
+        """Pages in use to the lowest numbers; tables dst follow."""
+        _check(lib().g3attn_pages_compact_device(self._h, _ref(pages), _ref(src), held, _ref(dst), status))

@@ -27,6 +27,7 @@
 #define LOG2E 1.4426950408889634f
 _Static_assert(G3ATTN_NOALLOC_MAX_HEADS == G3K_NOALLOC_MAX_HEADS, "fixed scratch size");
 #define G3_PROF_CAP 256
+#define G3_PG_BLOCKS 64
 #define D G3K_HEAD_DIM
 
 /* ------------------------------------------------------------------ errors */
@@ -167,6 +168,11 @@ struct g3attn_ctx {
      * only, and every layer inside the token forward (the default), 0 none
      * (G3ATTN_DECODE_NT) */
     int nt_loads;
+    /* scratch of the paged-cache calls: the block in use and the outgrown ones,
+     * kept because captured graphs hold their addresses */
+    void *d_pg, *pg_old[G3_PG_BLOCKS];
+    size_t d_pg_cap;
+    int pg_n_old;
     /* token forward: residual steps folded into the next GEMV's prologue
      * (bit 0: into the Q/K/V launch, bit 1: into the gate/up launch;
      * G3ATTN_FORWARD_FOLD) */
@@ -210,6 +216,8 @@ static void ctx_free(g3attn_ctx *c) {
     hipFree(c->d_logits);
     hipFree(c->d_pb);
     hipFree(c->d_tok);
+    hipFree(c->d_pg);
+    for (int i = 0; i < c->pg_n_old; i++) hipFree(c->pg_old[i]);
 
     if (c->h_logits) hipHostFree(c->h_logits);
     if (c->h_in) hipHostFree(c->h_in);
@@ -2290,4 +2298,326 @@ void g3attn_matvec_bf16(float *y, const uint16_t *A, const float *x, int M, int 
     pthread_mutex_lock(&g_gqa.lock);
     matvec_run(y, A, x, M, K);
     pthread_mutex_unlock(&g_gqa.lock);
+}
+
+/* ------------------------------------------------------------------ KV cache in pages */
+
+/* Scratch for one call.  An outgrown block stays allocated (queued calls and
+ * captured graphs use it); each new one is at least twice as large, so the
+ * blocks' sizes add up to less than twice the last one's. */
+static int paged_scratch(g3attn_ctx *c, size_t bytes, const char *fn, unsigned char **p) {
+    if (bytes > c->d_pg_cap) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(c->stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
+            set_err("%s: scratch memory cannot grow to %zu bytes while the stream is being captured", fn, bytes);
+            return G3_ERR_INVALID_ARG;
+        }
+        size_t cap = bytes > 2 * c->d_pg_cap ? bytes : 2 * c->d_pg_cap;
+        if (cap < (size_t)1 << 20) cap = (size_t)1 << 20;
+        void *d = NULL;
+        if (c->pg_n_old == G3_PG_BLOCKS) {
+            set_err("%s: too many scratch blocks", fn);
+            return G3_ERR_OUT_OF_MEMORY;
+        }
+        if (!alloc_dev(&d, cap, "paged scratch")) {
+            (void)hipGetLastError();
+            return G3_ERR_OUT_OF_MEMORY;
+        }
+        if (c->d_pg) c->pg_old[c->pg_n_old++] = c->d_pg;
+        c->d_pg = d;
+        c->d_pg_cap = cap;
+    }
+    *p = (unsigned char *)c->d_pg;
+    return G3_OK;
+}
+
+static int bad_arg(const char *fn, const char *what) {
+    set_err("%s: %s", fn, what);
+    return G3_ERR_INVALID_ARG;
+}
+
+#define PAGED_TRY(call)       \
+    do {                      \
+        int rc_ = (call);     \
+        if (rc_) return rc_;  \
+    } while (0)
+
+static int aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int log2i(int x) {
+    int n = 0;
+    while (x > 1) {
+        x >>= 1;
+        n++;
+    }
+    return n;
+}
+
+static int check_pages(const g3attn_ctx *c, const g3attn_pages *p, const char *fn) {
+    if (!c) return bad_arg(fn, "null context");
+    if (!p || !p->k || !p->v) return bad_arg(fn, "null pages");
+    if (p->dtype != G3ATTN_PAGE_F32 && p->dtype != G3ATTN_PAGE_BF16) return bad_arg(fn, "page dtype is neither G3ATTN_PAGE_F32 nor G3ATTN_PAGE_BF16");
+    if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+        return bad_arg(fn, "page_size is not a power of two from 16 to 1024");
+    if (p->num_pages < 1 || p->num_pages > (INT_MAX >> 1)) return bad_arg(fn, "num_pages out of range");
+    if (p->first_layer < 0 || p->num_layers < 1 || p->num_layers > 4096) return bad_arg(fn, "layers of the pages out of range");
+    if (!aligned16(p->k) || !aligned16(p->v)) return bad_arg(fn, "pages not 16-byte aligned");
+    const long long rows = (long long)c->cfg.num_kv_heads * p->page_size * D, most = 1LL << 31;
+    if (p->page_stride % 8 || p->page_stride < rows || p->page_stride > most) return bad_arg(fn, "page_stride too small or not a multiple of 8");
+    if (p->num_layers > 1) {
+        const long long s = p->layer_stride;
+        const int layers_apart = s <= most * p->num_pages && s >= (p->num_pages - 1) * p->page_stride + rows;
+        const int pages_apart = s >= rows && s <= most && p->page_stride >= (p->num_layers - 1) * s + rows;
+        if (s % 8 || (!layers_apart && !pages_apart && p->num_pages > 1) || s < rows)
+            return bad_arg(fn, "layer_stride lets layers' pages overlap, or is not a multiple of 8");
+    }
+    return G3_OK;
+}
+
+static int check_pages_layer(const g3attn_ctx *c, int layer, const g3attn_pages *p, const char *fn) {
+    PAGED_TRY(check_pages(c, p, fn));
+    if (!check_layer(c, layer, fn)) return G3_ERR_INVALID_ARG;
+    if (layer < p->first_layer || layer - p->first_layer >= p->num_layers) return bad_arg(fn, "the pages do not hold this layer");
+    return G3_OK;
+}
+
+static int check_seqs(const g3attn_pages *p, const g3attn_seqs *s, const char *fn) {
+    if (!s || !s->kv_len || !s->page_table) return bad_arg(fn, "null sequences");
+    if (s->num_seqs < 1 || s->num_seqs > G3K_PAGED_MAX_SEQS) return bad_arg(fn, "num_seqs is not from 1 to 4096");
+    if (s->table_stride < 1 || (long long)s->table_stride * p->page_size > G3K_PAGED_MAX_LEN)
+        return bad_arg(fn, "table_stride < 1, or table_stride * page_size > 2^24");
+    return G3_OK;
+}
+
+static int check_batch(const g3attn_pages *p, const g3attn_batch *b, const char *fn) {
+    if (!b) return bad_arg(fn, "null batch");
+    PAGED_TRY(check_seqs(p, &b->seqs, fn));
+    if (b->total_q < 0 || b->total_q > G3K_PAGED_MAX_LEN) return bad_arg(fn, "total_q is not from 0 to 2^24");
+    if (!b->q_start && b->total_q != b->seqs.num_seqs) return bad_arg(fn, "without q_start total_q has to be num_seqs");
+    return G3_OK;
+}
+
+static void fill_seqs(const g3attn_pages *p, const g3attn_batch *b, g3k_paged_seqs *s) {
+    s->kv_len = b->seqs.kv_len;
+    s->page_table = b->seqs.page_table;
+    s->q_start = b->q_start;
+    s->num_seqs = b->seqs.num_seqs;
+    s->table_stride = b->seqs.table_stride;
+    s->total_q = b->total_q;
+    s->page_shift = log2i(p->page_size);
+}
+
+static long long layer_bytes(const g3attn_pages *p, int layer) {
+    if (p->num_layers == 1) return 0;
+    return (long long)(layer - p->first_layer) * p->layer_stride * (p->dtype == G3ATTN_PAGE_BF16 ? 2 : 4);
+}
+
+int g3attn_paged_write_device(g3attn_ctx *c, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                              const float *Q, const float *K, const float *V, const uint16_t *q_norm,
+                              const uint16_t *k_norm, float *q_out) {
+    const char *fn = "g3attn_paged_write";
+    PAGED_TRY(check_pages_layer(c, layer, pages, fn));
+    PAGED_TRY(check_batch(pages, batch, fn));
+    if (!check_rope(c, fn)) return G3_ERR_INVALID_ARG;
+    if (batch->total_q == 0) return G3_OK;
+    if (!Q || !K || !V || !q_out) return bad_arg(fn, "null buffer");
+    if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(q_out)) return bad_arg(fn, "Q, K, V or q_out not 16-byte aligned");
+    if (!q_norm != !k_norm) return bad_arg(fn, "one of q_norm and k_norm without the other");
+    if (((uintptr_t)q_norm | (uintptr_t)k_norm) & 7) return bad_arg(fn, "norm gains not 8-byte aligned");
+    g3k_paged_write_args a;
+    memset(&a, 0, sizeof a);
+    fill_seqs(pages, batch, &a.s);
+    a.Q = Q;
+    a.K = K;
+    a.V = V;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.rope = g3attn_is_global_layer(layer) ? c->rope_global : c->rope_local;
+    a.eps = c->cfg.rmsnorm_eps;
+    a.q_out = q_out;
+    a.k = (char *)pages->k + layer_bytes(pages, layer);
+    a.v = (char *)pages->v + layer_bytes(pages, layer);
+    a.bf16 = pages->dtype == G3ATTN_PAGE_BF16;
+    a.num_pages = pages->num_pages;
+    a.n_kv_heads = c->cfg.num_kv_heads;
+    a.group = c->group;
+    a.max_context = c->max_context;
+    a.page_stride = pages->page_stride;
+    hipSetDevice(c->device);
+    const int rc = g3k_paged_write(&a, c->stream);
+    if (rc) return hip_fail((hipError_t)rc, "g3attn_paged_write launch");
+    return G3_OK;
+}
+
+static void fill_paged(g3attn_ctx *c, int layer, const g3attn_pages *pages, const g3attn_batch *batch, const float *q,
+                       float *out, g3k_paged_args *a) {
+    memset(a, 0, sizeof *a);
+    fill_seqs(pages, batch, &a->s);
+    a->k = (const char *)pages->k + layer_bytes(pages, layer);
+    a->v = (const char *)pages->v + layer_bytes(pages, layer);
+    a->bf16 = pages->dtype == G3ATTN_PAGE_BF16;
+    a->num_pages = pages->num_pages;
+    a->n_kv_heads = c->cfg.num_kv_heads;
+    a->group = c->group;
+    a->window = g3attn_is_global_layer(layer) ? INT_MAX / 2 : c->cfg.sliding_window;
+    if (a->window > INT_MAX / 2) a->window = INT_MAX / 2;
+    a->page_stride = pages->page_stride;
+    a->qscale = (1.0f / sqrtf((float)D)) * LOG2E;
+    a->q = q;
+    a->out = out;
+}
+
+static int check_attention(const float *q, const float *out, const char *fn) {
+    if (!q || !out) return bad_arg(fn, "null buffer");
+    if (!aligned16(q) || !aligned16(out)) return bad_arg(fn, "q or out not 16-byte aligned");
+    return G3_OK;
+}
+
+/* Row blocks of a packed batch, at most: `rows` rows (query heads of tokens)
+ * a block, and a part block for every sequence. */
+static int prefill_blocks(const g3attn_batch *b, int group, int rows) {
+    const int t = rows / group;
+    return b->total_q / t + (b->seqs.num_seqs < b->total_q ? b->seqs.num_seqs : b->total_q);
+}
+
+int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                                const float *q, float *out) {
+    const char *fn = "g3attn_paged_prefill";
+    PAGED_TRY(check_pages_layer(c, layer, pages, fn));
+    PAGED_TRY(check_batch(pages, batch, fn));
+    if (batch->total_q == 0) return G3_OK;
+    PAGED_TRY(check_attention(q, out, fn));
+    g3k_paged_args a;
+    fill_paged(c, layer, pages, batch, q, out, &a);
+    const int Hkv = c->cfg.num_kv_heads;
+    a.blocks = 1;
+    const int rows = 64 * a.blocks;
+    a.items = prefill_blocks(batch, c->group, rows);
+    /* few blocks: their keys are split until about two workgroups a CU are there */
+    long long parts = 2LL * c->n_cu / ((long long)a.items * Hkv);
+    a.parts = parts < 1 ? 1 : parts > 16 ? 16 : (int)parts;
+    hipSetDevice(c->device);
+    if (a.parts > 1) {
+        const size_t n = (size_t)a.items * a.parts * Hkv * rows, ob = align256(n * D * sizeof(float));
+        unsigned char *ws;
+        PAGED_TRY(paged_scratch(c, ob + n * 2 * sizeof(float), fn, &ws));
+        a.part_o = (float *)ws;
+        a.part_ml = (float *)(ws + ob);
+    }
+    const int rc = g3k_paged_prefill(&a, c->stream);
+    if (rc) return hip_fail((hipError_t)rc, "g3attn_paged_prefill launch");
+    return G3_OK;
+}
+
+int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                               const g3attn_prefixes *prefixes, const float *q, float *out) {
+    const char *fn = "g3attn_paged_decode";
+    PAGED_TRY(check_pages_layer(c, layer, pages, fn));
+    PAGED_TRY(check_batch(pages, batch, fn));
+    if (batch->q_start) return bad_arg(fn, "q_start set (one token per sequence; g3attn_paged_prefill takes more)");
+    PAGED_TRY(check_attention(q, out, fn));
+    g3k_paged_args a;
+    fill_paged(c, layer, pages, batch, q, out, &a);
+    const int Hkv = c->cfg.num_kv_heads, B = batch->seqs.num_seqs;
+    if (prefixes && prefixes->num_groups) {
+        if (prefixes->num_groups < 0 || prefixes->num_groups > B) return bad_arg(fn, "num_groups is not from 0 to num_seqs");
+        if (!prefixes->group_start || !prefixes->prefix_len) return bad_arg(fn, "null prefixes");
+        a.n_groups = prefixes->num_groups;
+        a.group_start = prefixes->group_start;
+        a.prefix_len = prefixes->prefix_len;
+    }
+    a.blocks = 1;
+    const int rows = 64 * a.blocks;
+    /* items per KV head: one workgroup a CU, and one more for every run of
+     * keys (its last chunk is a part one) */
+    const int units = B + (a.n_groups ? a.n_groups + B * c->group / rows : 0);
+    a.budget = units + (c->n_cu + Hkv - 1) / Hkv;
+    a.items = a.budget;
+    a.min_tiles = 2;
+    a.part_rows = a.n_groups ? rows : c->group;
+    const size_t n = (size_t)a.items * Hkv * a.part_rows, ob = align256(n * D * sizeof(float)), mb = align256(n * 2 * sizeof(float));
+    hipSetDevice(c->device);
+    unsigned char *ws;
+    PAGED_TRY(paged_scratch(c, ob + mb + (size_t)B * 4 * sizeof(int), fn, &ws));
+    a.part_o = (float *)ws;
+    a.part_ml = (float *)(ws + ob);
+    a.dir_prefix = (int *)(ws + ob + mb);
+    a.dir_tail = a.dir_prefix + 2 * B;
+    const int rc = g3k_paged_decode(&a, c->stream);
+    if (rc) return hip_fail((hipError_t)rc, "g3attn_paged_decode launch");
+    return G3_OK;
+}
+
+static void fill_pages(const g3attn_ctx *c, const g3attn_pages *p, const g3attn_seqs *from, const g3attn_seqs *to,
+                       const int *held, int *status, g3k_pages_args *a) {
+    memset(a, 0, sizeof *a);
+    a->k = p->k;
+    a->v = p->v;
+    a->elem = p->dtype == G3ATTN_PAGE_BF16 ? 2 : 4;
+    a->num_layers = p->num_layers;
+    a->num_pages = p->num_pages;
+    a->page_shift = log2i(p->page_size);
+    a->n_kv_heads = c->cfg.num_kv_heads;
+    a->table_stride = from->table_stride;
+    a->page_stride = p->page_stride;
+    a->layer_stride = p->num_layers > 1 ? p->layer_stride : 0;
+    a->n_in = from->num_seqs;
+    a->n_out = to->num_seqs;
+    a->len_in = from->kv_len;
+    a->table_in = from->page_table;
+    a->len_out = to->kv_len;
+    a->table_out = to->page_table;
+    a->held = held;
+    a->status = status;
+}
+
+int g3attn_pages_fork_device(g3attn_ctx *c, const g3attn_pages *pages, const g3attn_seqs *from, const int *parent,
+                             const int *add, const int *held, const g3attn_seqs *to, int *status) {
+    const char *fn = "g3attn_pages_fork";
+    PAGED_TRY(check_pages(c, pages, fn));
+    PAGED_TRY(check_seqs(pages, from, fn));
+    PAGED_TRY(check_seqs(pages, to, fn));
+    if (from->table_stride != to->table_stride) return bad_arg(fn, "from and to have different table_strides");
+    g3k_pages_args a;
+    fill_pages(c, pages, from, to, held, status, &a);
+    a.parent = parent;
+    a.add = add;
+    hipSetDevice(c->device);
+    const size_t n = align256((size_t)a.num_pages * sizeof(int)), rb = align256((size_t)a.n_out * a.table_stride * sizeof(int));
+    unsigned char *ws;
+    PAGED_TRY(paged_scratch(c, 4 * n + rb + (size_t)a.n_out * sizeof(g3k_fork_child), fn, &ws));
+    a.ref = (int *)ws;
+    a.writers = (int *)(ws + n);
+    a.first = (int *)(ws + 2 * n);
+    a.list = (int *)(ws + 3 * n);
+    a.rows = (int *)(ws + 4 * n);
+    a.child = (g3k_fork_child *)(ws + 4 * n + rb);
+    const int rc = g3k_pages_fork(&a, c->stream);
+    if (rc) return hip_fail((hipError_t)rc, "g3attn_pages_fork launch");
+    return G3_OK;
+}
+
+int g3attn_pages_compact_device(g3attn_ctx *c, const g3attn_pages *pages, const g3attn_seqs *from, const int *held,
+                                const g3attn_seqs *to, int *status) {
+    const char *fn = "g3attn_pages_compact";
+    PAGED_TRY(check_pages(c, pages, fn));
+    PAGED_TRY(check_seqs(pages, from, fn));
+    PAGED_TRY(check_seqs(pages, to, fn));
+    if (from->table_stride != to->table_stride || from->num_seqs != to->num_seqs)
+        return bad_arg(fn, "from and to have different num_seqs or table_strides");
+    g3k_pages_args a;
+    fill_pages(c, pages, from, to, held, status, &a);
+    hipSetDevice(c->device);
+    const size_t n = align256((size_t)a.num_pages * sizeof(int));
+    unsigned char *ws;
+    PAGED_TRY(paged_scratch(c, 4 * n + sizeof(int), fn, &ws));
+    a.ref = (int *)ws;
+    a.list = (int *)(ws + n);
+    a.list2 = (int *)(ws + 2 * n);
+    a.map = (int *)(ws + 3 * n);
+    a.count = (int *)(ws + 4 * n);
+    a.copy_wgs = 8 * c->n_cu;
+    const int rc = g3k_pages_compact(&a, c->stream);
+    if (rc) return hip_fail((hipError_t)rc, "g3attn_pages_compact launch");
+    return G3_OK;
 }

@@ -336,6 +336,148 @@ int g3attn_matmul_bf16_device(g3attn_ctx *ctx, float *C, const uint16_t *W, cons
 int g3attn_prefill_forward_device(g3attn_ctx *ctx, const g3attn_weights *weights, const int *tokens,
                                   int num_tokens, int start_pos, float *logits);
 
+/* ---- KV cache in pages: many sequences at once ----
+ *
+ * For engines that serve several conversations from one model (no counterpart
+ * in the reference, which holds one).  The caller owns the memory: a pool of
+ * pages, a table of page numbers and a length per sequence, all on the
+ * device, so that a serving loop can be enqueued, or captured into a graph,
+ * without the host reading anything back.  The calls:
+ *   g3attn_pages_fork_device      fork, extend, roll back and end sequences
+ *   g3attn_paged_write_device     QK-norm + RoPE of new tokens, K / V to pages
+ *   g3attn_paged_prefill_device   causal attention of packed new tokens
+ *   g3attn_paged_decode_device    one token per sequence, shared prefixes
+ *   g3attn_pages_compact_device   pages in use to the lowest numbers
+ * A step of a serving loop is a fork (which gives each sequence room for its
+ * new tokens), then per layer a write and a prefill or decode.
+ *
+ * All pointers are device memory, everything is enqueued on the context's
+ * stream (g3attn_stream) of the context's device, and memory used on another
+ * stream has to be ordered against it by the caller.  What the device arrays
+ * hold cannot be refused; it is kept within the buffers instead: a length
+ * counts as at most table_stride * page_size and at least 0, row offsets as
+ * within [0, total_q], group bounds as within [0, num_seqs].  A page number
+ * outside [0, num_pages) is never followed: attention leaves its positions
+ * out, writes to it are dropped.
+ *
+ * Scratch memory belongs to the context and grows with the largest call; a
+ * call that would have to grow it while the stream is being captured returns
+ * -1 (make one call of that size before).  Growing leaves the old memory
+ * allocated until the context is destroyed, so graphs captured earlier stay
+ * valid; graphs of one context share the scratch, so no two of them, and no
+ * other call of the context, may run at the same time. */
+
+#define G3ATTN_PAGE_F32 0
+#define G3ATTN_PAGE_BF16 1   /* rounded to nearest even when written */
+
+/* A pool of pages for model layers first_layer .. first_layer + num_layers - 1.
+ * Page p of a layer holds rows [num_kv_heads][page_size][256] of K (and of V)
+ * at k + (layer - first_layer) * layer_stride + p * page_stride elements.
+ * page_size: a power of two, 16 to 1024.  Strides: multiples of 8 elements,
+ * pages of all layers apart from each other (layer after layer, or page after
+ * page); layer_stride is not read with one layer.  k and v 16-byte aligned. */
+typedef struct {
+    void *k, *v;
+    int dtype;
+    int first_layer, num_layers;
+    int num_pages, page_size;
+    long long page_stride, layer_stride;
+} g3attn_pages;
+
+/* Sequences in a pool: their lengths kv_len [num_seqs] and the pages of their
+ * positions, page_table [num_seqs][table_stride] (entry j: positions
+ * j * page_size ..).  Up to 4096 sequences, table_stride * page_size up to
+ * 2^24. */
+typedef struct {
+    int num_seqs;
+    int *kv_len;
+    int *page_table;
+    int table_stride;
+} g3attn_seqs;
+
+/* New tokens of sequences, packed: sequence b's are rows q_start[b] ..
+ * q_start[b + 1] - 1 (ascending, [num_seqs + 1]; any number, zero too), the
+ * last ones of its kv_len positions.  q_start NULL: one token per sequence,
+ * total_q = num_seqs.  total_q is the number of rows the buffers hold, up to
+ * 2^24; rows behind the last sequence's are not read, and not written. */
+typedef struct {
+    g3attn_seqs seqs;
+    int total_q;
+    const int *q_start;
+} g3attn_batch;
+
+/* Prefixes that runs of sequences share: sequences group_start[i] ..
+ * group_start[i + 1] - 1 (ascending, [num_groups + 1]) hold the same keys and
+ * values at positions 0 .. prefix_len[i] - 1, not more than any of them has.
+ * They are read from the first one's pages.  Sequences in no group share
+ * nothing. */
+typedef struct {
+    int num_groups;
+    const int *group_start;
+    const int *prefix_len;
+} g3attn_prefixes;
+
+/* The front half of a layer's attention for packed tokens: QK-norm (q_norm and
+ * k_norm bf16 [256], both NULL: none) and RoPE at each token's position, with
+ * the layer's table; q to q_out [total_q][num_heads * 256] (may be Q itself),
+ * K (normed, rotated) and V to the token's row of its page.  Q
+ * [total_q][num_heads * 256], K, V [total_q][num_kv_heads * 256], fp32.  A
+ * page that is written may not be another sequence's too
+ * (g3attn_pages_fork_device sees to that).  Tokens at positions from the
+ * context's max_context on, or below 0, are left out: nothing of theirs is
+ * written. */
+int g3attn_paged_write_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                              const float *Q, const float *K, const float *V, const uint16_t *q_norm,
+                              const uint16_t *k_norm, float *q_out);
+
+/* Causal attention of packed tokens over their sequences' pages, their own
+ * keys included (written before): q as g3attn_paged_write_device leaves it,
+ * out [total_q][num_heads * 256].  The token at position p sees positions
+ * [0, p], or [p - sliding_window + 1, p] on a local layer.  A token that sees
+ * no key gets zeros.  Scores and products hold 22 bits of q, K, V and the
+ * probabilities, with fp32 sums: about 3e-7 of the output's RMS (keys that
+ * are seen have to be finite).  The result does not depend on what else is in
+ * the batch beyond the order of sums. */
+int g3attn_paged_prefill_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                                const float *q, float *out);
+
+/* The same for one token per sequence (batch->q_start NULL), at position
+ * kv_len - 1.  prefixes (may be NULL): runs of sequences whose first positions
+ * are the same; the shared keys are read and multiplied once for all of a
+ * run.  The result is that of the call without prefixes, up to the order of
+ * sums. */
+int g3attn_paged_decode_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
+                               const g3attn_prefixes *prefixes, const float *q, float *out);
+
+/* New sequences from old ones, in one pass over tables: sequence b of `to`
+ * continues sequence parent[b] of `from` (parent NULL: sequence b), cut or
+ * grown by add[b] positions (add NULL: 0; below 0: the last ones are dropped);
+ * a parent outside `from` gives an empty sequence.  Pages are shared: to's
+ * table names the parent's pages.  A page that b will write next, the partial
+ * last one of a sequence that grows, becomes its own: unless everyone who has
+ * it grows too and b is the first of them, its rows are copied to a new page,
+ * in K and V of every layer.  Pages of positions beyond are new; entries
+ * beyond the length are -1.  Sequences of `from` that are nobody's parent
+ * end: pages that `to` does not name are free.  So `from` has to name
+ * every page in use, or the caller to hold it: held [num_pages] (may be NULL),
+ * nonzero for pages that are neither given out nor changed.  New pages are the
+ * lowest free ones, to sequences in order.  If they run out, or a table row
+ * is too short, a sequence keeps its parent's length (its new positions are
+ * not there).  status (may be NULL): [0] pages in use afterwards, held ones
+ * included, [1] sequences that were not grown.  `to` may be `from` (same
+ * arrays); both have one table_stride. */
+int g3attn_pages_fork_device(g3attn_ctx *ctx, const g3attn_pages *pages, const g3attn_seqs *from, const int *parent,
+                             const int *add, const int *held, const g3attn_seqs *to, int *status);
+
+/* Moves the pages in use to the lowest numbers, so that the rest of the pool
+ * can be given up: of n pages in use, those numbered n and up move, in order,
+ * into the free ones below, K and V of every layer; tables follow (`to` may be
+ * `from`; same num_seqs and table_stride), entries beyond a length become -1.
+ * Held pages (as above) count as in use and do not move.  status (may be
+ * NULL): [0] pages in use, [1] pages moved. */
+int g3attn_pages_compact_device(g3attn_ctx *ctx, const g3attn_pages *pages, const g3attn_seqs *from, const int *held,
+                                const g3attn_seqs *to, int *status);
+
 /* The context's HIP stream (hipStream_t), for callers that interleave their
  * own work; and a wait for everything queued on it. */
 void *g3attn_stream(g3attn_ctx *ctx);

@@ -39,6 +39,18 @@
 //   profile kind       (g3attn_profile_enable, or once enabled
 //                    g3attn_profile_read: prints "profile <kind> <ms> <count>")
 //   destroy
+//   pool bf16 first_layer num_layers num_pages page_size page_stride
+//        layer_stride K V               (the pages; raw fp32 or bf16 arrays)
+//   pool_out K V
+//   seqs slot num_seqs table_stride kv_len page_table   (slots 0 .. 3)
+//   seqs_out slot kv_len page_table
+//   paged_write layer slot total_q q_start|- Q K V q_norm|- k_norm|- q_out
+//   paged_prefill layer slot total_q q_start|- q out
+//   paged_decode layer slot num_groups group_start|- prefix_len|- q out
+//   pages_fork from parent|- add|- held|- to status     (slots)
+//   pages_compact from held|- to status
+//                    (all of these with device copies; outputs hold what the
+//                    named file holds before the call where it exists)
 //   front_stage_only Hkv nk V vt_out            (g3k_rope_write_stage with an
 //                    empty batch, ra.n = 0, and no cache: the V^T staging of
 //                    nk keys alone; vt_out gets the bf16 hi plane [Hkv][256][ldk])
@@ -148,6 +160,30 @@ struct Model {
     }
 };
 
+// The paged cache of the script: pages, and sequences in slots.
+struct Paged {
+    g3attn_pages pages{};
+    size_t bytes = 0;
+    g3attn_seqs seqs[4]{};
+    std::vector<void *> dev;
+    template <typename T>
+    T *put(const std::string &name) {
+        if (name == "-") return nullptr;
+        T *p = to_device(read_bin<T>(name, file_elems(name, sizeof(T))));
+        dev.push_back(p);
+        return p;
+    }
+    // An output of n values: what the file holds, or a marker.
+    float *out(const std::string &name, size_t n) {
+        float *p = to_device(exists(name) ? read_bin<float>(name, n) : std::vector<float>(n, -12345.0f));
+        dev.push_back(p);
+        return p;
+    }
+    ~Paged() {
+        for (void *p : dev) hipFree(p);
+    }
+};
+
 void check(int rc, const std::string &call) {
     if (rc) {
         std::fprintf(stderr, "attn_emu: %s returned %d: %s\n", call.c_str(), rc, g3attn_last_error());
@@ -166,6 +202,7 @@ int main(int argc, char **argv) {
     bool profiling = false;
     int H = 0, Hkv = 0, layers = 0, hidden = 0, vocab = 0;
     Model *model = nullptr;
+    Paged paged;
     const size_t D = 256;
     std::string line;
     while (std::getline(script, line)) {
@@ -199,6 +236,87 @@ int main(int argc, char **argv) {
                 std::fprintf(stderr, "attn_emu: g3attn_create failed: %s\n", g3attn_last_error());
                 return 1;
             }
+        } else if (cmd == "pool") {
+            int bf16;
+            std::string kf, vf;
+            g3attn_pages &p = paged.pages;
+            in >> bf16 >> p.first_layer >> p.num_layers >> p.num_pages >> p.page_size >> p.page_stride >> p.layer_stride >> kf >> vf;
+            if (!in) die("bad pool line");
+            p.dtype = bf16 ? G3ATTN_PAGE_BF16 : G3ATTN_PAGE_F32;
+            paged.bytes = file_elems(kf, 1);
+            p.k = paged.put<unsigned char>(kf);
+            p.v = paged.put<unsigned char>(vf);
+        } else if (cmd == "pool_out") {
+            std::string kf, vf;
+            in >> kf >> vf;
+            write_bin(kf, static_cast<unsigned char *>(paged.pages.k), paged.bytes);
+            write_bin(vf, static_cast<unsigned char *>(paged.pages.v), paged.bytes);
+        } else if (cmd == "seqs") {
+            int slot;
+            std::string lf, tf;
+            g3attn_seqs x{};
+            in >> slot >> x.num_seqs >> x.table_stride >> lf >> tf;
+            if (!in || slot < 0 || slot > 3) die("bad seqs line");
+            x.kv_len = paged.put<int>(lf);
+            x.page_table = paged.put<int>(tf);
+            paged.seqs[slot] = x;
+        } else if (cmd == "seqs_out") {
+            int slot;
+            std::string lf, tf;
+            in >> slot >> lf >> tf;
+            const g3attn_seqs &x = paged.seqs[slot];
+            write_bin(lf, x.kv_len, (size_t)x.num_seqs);
+            write_bin(tf, x.page_table, (size_t)x.num_seqs * x.table_stride);
+        } else if (cmd == "paged_write" || cmd == "paged_prefill") {
+            int layer, slot, n;
+            std::string sf, qf, kf, vf, qn, kn, of;
+            in >> layer >> slot >> n >> sf >> qf;
+            const bool write = cmd == "paged_write";
+            if (write) in >> kf >> vf >> qn >> kn;
+            in >> of;
+            if (!in) die("bad " + cmd + " line");
+            g3attn_batch b{paged.seqs[slot], n, paged.put<int>(sf)};
+            const size_t cnt = (size_t)n * H * D;
+            const float *q = paged.put<float>(qf);
+            float *out = paged.out(of, cnt);
+            if (write) {
+                const float *k = paged.put<float>(kf), *v = paged.put<float>(vf);
+                check(g3attn_paged_write_device(ctx, layer, &paged.pages, &b, q, k, v, paged.put<uint16_t>(qn),
+                                                paged.put<uint16_t>(kn), out), cmd);
+            } else {
+                check(g3attn_paged_prefill_device(ctx, layer, &paged.pages, &b, q, out), cmd);
+            }
+            write_bin(of, out, cnt);
+        } else if (cmd == "paged_decode") {
+            int layer, slot, groups;
+            std::string gf, pf, qf, of;
+            in >> layer >> slot >> groups >> gf >> pf >> qf >> of;
+            if (!in) die("bad paged_decode line");
+            g3attn_batch b{paged.seqs[slot], paged.seqs[slot].num_seqs, nullptr};
+            const g3attn_prefixes pr{groups, paged.put<int>(gf), paged.put<int>(pf)};
+            const size_t cnt = (size_t)b.total_q * H * D;
+            const float *q = paged.put<float>(qf);
+            float *out = paged.out(of, cnt);
+            check(g3attn_paged_decode_device(ctx, layer, &paged.pages, &b, groups < 0 ? nullptr : &pr, q, out), cmd);
+            write_bin(of, out, cnt);
+        } else if (cmd == "pages_fork" || cmd == "pages_compact") {
+            int from, to;
+            std::string pf, af, hf, sf;
+            const bool fork = cmd == "pages_fork";
+            in >> from;
+            if (fork) in >> pf >> af;
+            in >> hf >> to >> sf;
+            if (!in) die("bad " + cmd + " line");
+            int *status = to_device(std::vector<int>(2, -12345));
+            paged.dev.push_back(status);
+            const int *held = paged.put<int>(hf);
+            if (fork) {
+                const int *parent = paged.put<int>(pf), *add = paged.put<int>(af);
+                check(g3attn_pages_fork_device(ctx, &paged.pages, &paged.seqs[from], parent, add, held, &paged.seqs[to], status), cmd);
+            } else {
+                check(g3attn_pages_compact_device(ctx, &paged.pages, &paged.seqs[from], held, &paged.seqs[to], status), cmd);
+            }
+            write_bin(sf, status, 2);
         } else if (cmd == "kv_write" || cmd == "kv_read") {
             int layer, slot, n;
             std::string kf, vf;

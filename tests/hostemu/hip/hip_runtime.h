@@ -269,6 +269,17 @@ inline void __threadfence() {}
 #ifndef __HIP_MEMORY_SCOPE_WORKGROUP
 #define __HIP_MEMORY_SCOPE_WORKGROUP 3
 #endif
+inline void __threadfence_block() {}
+inline int atomicAdd(int *p, int v) {
+    const int old = *p;
+    *p = old + v;
+    return old;
+}
+inline int atomicMin(int *p, int v) {
+    const int old = *p;
+    if (v < old) *p = v;
+    return old;
+}
 inline unsigned atomicInc(unsigned *p, unsigned v) {
     const unsigned old = *p;
     *p = old >= v ? 0u : old + 1u;
@@ -345,6 +356,12 @@ inline float __shfl(float v, int src) {
     hostemu::exchange(__float_as_uint(v), 0, src, &r, &unused);
     return __uint_as_float(r);
 }
+
+// The integer forms.
+inline int __shfl_xor(int v, int mask, int width = 64) {
+    return __float_as_int(__shfl_xor(__int_as_float(v), mask, width));
+}
+inline int __shfl(int v, int src) { return __float_as_int(__shfl(__int_as_float(v), src)); }
 
 inline float hostemu_exp2f(float x) { return exp2f(x); }
 #define __builtin_amdgcn_exp2f hostemu_exp2f

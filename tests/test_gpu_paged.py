@@ -1,0 +1,199 @@
+"""The paged-cache entry points on the GPU against 64-bit oracles
+(paged_cases.py, which derives the tolerances): every head layout, page type and
+size, lengths from nothing to thousands, spoiled tables, refusals, a serving
+loop of all of them, and graph replays."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_cases as P
+from helpers import DeviceBuffer
+
+pytestmark = pytest.mark.gpu
+
+GLOBAL, LOCAL = 5, 0
+HEADS = [(8, 4), (16, 8), (4, 1), (4, 4)]
+
+
+@pytest.fixture
+def run():
+    made = []
+
+    def make(**kw):
+        made.append(P.GpuRunner(**kw))
+        return made[-1]
+    yield make
+    for r in made:
+        r.done()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_write(run, hq, hkv, bf16):
+    r = run(hq=hq, hkv=hkv, max_context=400)
+    P.run_write(r, LOCAL, [5, 0, 1, 117], [21, 4, 390, 117], 16, bf16, padding=2)
+    P.run_write(r, GLOBAL - 1, [3, 4], [90, 4], 32, bf16, norm=False, seed=1, pool_kw=dict(order="pages", pad=8), label="no norm")
+    P.run_write(r, LOCAL, [1] * 70, list(range(1, 71)), 64, bf16, seed=2, label="steps")
+    P.run_write(r, LOCAL, [20, 9, 3], [20, 405, 1], 16, bf16, seed=3, bad=[(0, 0, -1), (1, 1, 500)], label="outside")
+    P.run_write(r, LOCAL, [0, 0, 2] + [0] * 90 + [3], [0, 5, 2] + [1] * 90 + [3], 16, bf16, seed=4, label="empty ones")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_prefill(run, hq, hkv, bf16):
+    r = run(hq=hq, hkv=hkv, window=100, max_context=1024)
+    P.run_prefill(r, GLOBAL, [37, 0, 1, 120], [37, 5, 50, 261], 16, bf16, padding=3)
+    P.run_prefill(r, LOCAL, [190, 40], [260, 40], 32, bf16, seed=1, label="local")
+    P.run_prefill(r, GLOBAL, [5, 9, 7], [50, 33, 7], 16, bf16, seed=2, bad=[(0, 1, -1), (1, 0, 999), (1, 1, -7), (1, 2, 1 << 30)],
+                  label="absent")
+    P.run_prefill(r, LOCAL, [12, 3], [5, 0], 128, bf16, seed=3, label="short")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layer", [GLOBAL, LOCAL])
+def test_prefill_long(run, layer, bf16):
+    """Histories of thousands, and blocks enough to fill the chip."""
+    r = run(window=1024, max_context=4096)
+    P.run_prefill(r, layer, [3, 140], [3001, 2111], 64, bf16, label="history")
+    r2 = run(hq=4, hkv=4, window=512)
+    P.run_prefill(r2, layer, [300] * 14 + [1] * 30, [300] * 14 + list(range(1, 31)), 16, bf16, seed=1, label="many")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_scales(run, bf16):
+    r = run(hq=2, hkv=1)
+    for i, (qs, ks) in enumerate([(2e6, 1e-6), (1e-9, 3e8), (0.0, 1.0)]):
+        P.run_prefill(r, GLOBAL, [6], [45], 16, bf16, seed=i, scale=qs, kv_scale=ks, label=f"q {qs} kv {ks}")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_decode(run, hq, hkv, bf16):
+    r = run(hq=hq, hkv=hkv, window=300, max_context=8192)
+    P.run_decode(r, GLOBAL, [1] * 5, [0] * 5, [1, 2, 33, 700, 16], 16, bf16, groups=False)
+    P.run_decode(r, GLOBAL, [3, 1, 2], [400, 9, 0], [1, 5, 300, 3, 8, 2], 16, bf16, seed=1, label="groups")
+    P.run_decode(r, LOCAL, [3, 2], [400, 17], [1, 500, 12, 3, 20], 32, bf16, seed=2, label="groups, local")
+    P.run_decode(r, GLOBAL, [70, 3], [135, 64], [1 + i % 50 for i in range(73)], 16, bf16, seed=3, label="many members")
+    P.run_decode(r, GLOBAL, [2], [2000], [3000, 0], 64, bf16, seed=4, label="long")
+    P.run_decode(r, GLOBAL, [1, 1, 1], [0, 0, 0], [0, 7, 0], 16, bf16, seed=5, groups=False, label="empty")
+    P.run_decode(r, GLOBAL, [2, 1], [30, 0], [40, 3, 60], 16, bf16, seed=6, bad=[(0, 3, -1), (2, 1, 77), (2, 0, -9)], label="absent")
+
+
+def test_decode_malformed_groups(run):
+    """Group bounds and row offsets that overlap or run backwards stay inside the
+    buffers, as on the emulated machine."""
+    r = run(hq=2, hkv=1)
+    rng = np.random.default_rng(0)
+    lens, ps = [40, 50, 33, 20], 16
+    table = P.tables_for(rng, lens, ps, 16)
+    pool = P.Pool(rng, 1, 16, 1, ps, False, first_layer=GLOBAL)
+    pool.fill(rng, table, lens)
+    q = rng.standard_normal((4, 2, P.D)).astype(np.float32)
+    r.pool(pool)
+    r.seqs(0, lens, table)
+    for groups in [([0, 9, -4, 4], [30, 1 << 30, 20]), ([3, 0, 4, 0], [5, 6, 7]), ([-5, 4, 0, 4], [-3, 33, 20])]:
+        r.decode(GLOBAL, 0, groups, q, lambda out: None)
+    r.prefill(GLOBAL, 0, [0, 3, 1, 9, 2], q, lambda out: None)
+    r.prefill(GLOBAL, 0, [-7, 2, 2, -1, 1 << 30], q, lambda out: None)
+
+
+def test_many_sequences(run):
+    """More sequences than a wave looks at in one go, most of them short."""
+    r = run(hq=4, hkv=1, max_context=2048)
+    n = 300
+    P.run_decode(r, GLOBAL, [1] * n, [0] * n, [1 + (7 * i) % 40 for i in range(n)], 16, True, groups=False, label="300 sequences")
+    P.run_decode(r, GLOBAL, [30] * 10, [20 + 3 * i for i in range(10)], [1 + (7 * i) % 40 for i in range(n)], 16, False, seed=1, label="10 groups")
+    P.run_prefill(r, GLOBAL, [i % 3 for i in range(n)], [i % 3 + i % 20 for i in range(n)], 16, False, seed=2, label="300 prompts")
+
+
+def test_fork(run):
+    r = run(hq=2, hkv=2)
+    _, _, st, copies = P.run_fork(r, [20, 33, 16, 7], [0, 0, 3, -1, 1], [1, 1, 1, 1, 0], 16, 16)
+    assert len(copies) == 1 and st[1] == 0
+    P.run_fork(r, [32, 20], [0, 0, 1, 1, 1], [1, 17, 0, 5, 40], 16, 24, bf16=True, seed=1, stride=6, label="mixed")
+    P.run_fork(r, [40, 20, 9], [0, 1, 2, 7], [-10, -40, -9, 3], 16, 12, seed=2, label="rollback")
+    P.run_fork(r, [5, 16, 31], [0, 1, 2], [1, 1, 1], 16, 9, seed=3, alias=True, label="step")
+    P.run_fork(r, [5, 16, 31], [0, 1, 2], [0, 0, 0], 16, 9, seed=3, null=("parent", "add"), label="identity")
+    P.run_fork(r, [20, 33, 16, 7], [3, 0, 0, 1], [1, 1, 1, 1], 16, 16, seed=4, alias=True, label="reordered in place")
+    _, _, st, _ = P.run_fork(r, [30, 30], [0, 0, 1, 1], [1, 1, 40, 3], 16, 6, stride=4, label="short")
+    assert st[1] > 0
+    P.run_fork(r, [30, 30], [0, 1], [40, 2], 16, 9, seed=1, stride=4, label="row")
+    held = np.zeros(20, np.int32)
+    held[[0, 1, 5, 19]] = 1
+    P.run_fork(r, [20, 40], [0, 1, 1], [3, 30, 1], 16, 20, held=held, seed=2, stride=8, label="held")
+    P.run_fork(r, [20, 40, 18], [0, 1, 2], [3, 30, 5], 16, 20, held=held, seed=3, stride=8, bad=[(0, 1, 5), (1, 0, -3), (2, 1, 1 << 20)],
+               label="held tail")
+    P.run_fork(r, [36, 40, 33], [2, 0, 1, 1], [1, 0, 2, 9], 16, 20, seed=4, shared=[(0, 3, 2)], label="shared")
+    rng = np.random.default_rng(5)
+    P.run_fork(r, list(rng.integers(0, 90, 400)), list(rng.integers(-1, 401, 3000)), list(rng.integers(-3, 40, 3000)), 16, 5003, seed=6,
+               layers=1, stride=9, label="many")
+
+
+def test_compact(run):
+    r = run(hq=2, hkv=1)
+    P.run_compact(r, [20, 33, 0, 16, 1], 16, 30)
+    P.run_compact(r, [20, 33], 16, 30, bf16=True, seed=1, alias=True, label="in place", pool_kw=dict(order="pages", pad=8))
+    P.run_compact(r, [40, 40, 45], 16, 64, seed=2, shared=[(0, 3, 2)], label="shared")
+    held = np.zeros(70, np.int32)
+    held[[0, 3, 40, 69]] = 1
+    P.run_compact(r, [40, 40, 45], 16, 70, held=held, seed=3, label="held")
+    P.run_compact(r, [40, 40], 16, 20, seed=3, bad=[(0, 1, -1), (1, 2, 1 << 30)], label="absent")
+    P.run_compact(r, [0, 0], 16, 20, seed=4, label="empty")
+    P.run_compact(r, [16] * 2000, 16, 9001, seed=5, layers=1, label="large")
+
+
+def test_refusals(run):
+    """What the host can see is refused with a message before anything is enqueued."""
+    r = run(hq=4, hkv=2, layers=6)
+    G, ctx = r.G, r.ctx
+    A = 1 << 40      # never followed: each call is refused first
+
+    def pages(**kw):
+        d = dict(k=A, v=A, dtype=G.PAGE_F32, first_layer=0, num_layers=6, num_pages=8, page_size=16, page_stride=2 * 16 * 256,
+                 layer_stride=8 * 2 * 16 * 256)
+        d.update(kw)
+        return G.Pages(**d)
+
+    def seqs(**kw):
+        d = dict(num_seqs=2, kv_len=A, page_table=A, table_stride=4)
+        d.update(kw)
+        return G.Seqs(**d)
+
+    def batch(total=7, start=A, **kw):
+        return G.Batch(seqs=seqs(**kw), total_q=total, q_start=start)
+
+    def refused(f, *a):
+        with pytest.raises(G.G3AttnError) as e:
+            f(*a)
+        assert e.value.rc == G.ERR_INVALID_ARG and str(e.value)
+    for bad in (dict(k=None), dict(v=None), dict(dtype=2), dict(page_size=24), dict(page_size=8), dict(page_size=2048), dict(num_pages=0),
+                dict(num_layers=0), dict(first_layer=-1), dict(page_stride=2 * 16 * 256 - 8), dict(page_stride=2 * 16 * 256 + 4),
+                dict(layer_stride=8), dict(k=A + 4), dict(layer_stride=7 * 2 * 16 * 256)):
+        refused(ctx.paged_prefill_device, 0, pages(**bad), batch(), A, A)
+        refused(ctx.pages_compact_device, pages(**bad), seqs(), None, seqs())
+    for layer, first in ((6, 0), (-1, 0), (0, 1), (5, 6)):
+        refused(ctx.paged_prefill_device, layer, pages(first_layer=first), batch(), A, A)
+    for bad in (dict(num_seqs=0), dict(num_seqs=4097), dict(kv_len=None), dict(page_table=None), dict(table_stride=0), dict(table_stride=1 << 21)):
+        refused(ctx.paged_write_device, 0, pages(), batch(**bad), A, A, A, None, None, A)
+        refused(ctx.paged_decode_device, 0, pages(), batch(2, None, **bad), None, A, A)
+        refused(ctx.pages_fork_device, pages(), seqs(**bad), None, None, None, seqs())
+        refused(ctx.pages_fork_device, pages(), seqs(), None, None, None, seqs(**bad))
+    for b in (batch(-1), batch((1 << 24) + 1), batch(3, None), None):
+        refused(ctx.paged_prefill_device, 0, pages(), b, A, A)
+    for a in ((None, A, A, A), (A, None, A, A), (A, A, None, A), (A, A, A, None), (A + 4, A, A, A)):
+        refused(ctx.paged_write_device, 0, pages(), batch(), *a[:3], None, None, a[3])
+    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A, None, A)
+    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A + 2, A, A)
+    refused(ctx.paged_prefill_device, 0, pages(), batch(), None, A)
+    refused(ctx.paged_prefill_device, 0, pages(), batch(), A, A + 8)
+    refused(ctx.paged_decode_device, 0, pages(), batch(), None, A, A)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=3, group_start=A, prefix_len=A), A, A)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=1, group_start=None, prefix_len=A), A, A)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=-1, group_start=A, prefix_len=A), A, A)
+    refused(ctx.pages_fork_device, pages(), seqs(), None, None, None, seqs(table_stride=5))
+    refused(ctx.pages_compact_device, pages(), seqs(), None, seqs(num_seqs=3))
+    assert G.lib().g3attn_paged_prefill_device(None, 0, C.byref(pages()), C.byref(batch()), A, A) == G.ERR_INVALID_ARG
+    ctx.paged_prefill_device(0, pages(), batch(0), None, None)      # nothing to do
+    with G.Context(G.default_config(num_layers=1, max_context=16), 16, defer_rope=True) as bare:
+        refused(bare.paged_write_device, 0, pages(num_layers=1, page_stride=4 * 16 * 256), batch(), A, A, A, None, None, A)
