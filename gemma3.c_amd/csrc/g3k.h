@@ -391,12 +391,14 @@ typedef struct {
 int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
 
 /* Attention of packed tokens (prefill) or of one token per sequence (decode)
- * over pages; q and out [total_q][heads][D].  blocks: 16-row blocks per wave
- * (1 or 2: 64 or 128 rows per workgroup).
- * Prefill: items bounds the row blocks of the batch, sum over sequences of
- * ceil(tokens * group / (64 blocks)); each block's keys go to up to `parts`
- * workgroups, whose parts [items][parts][n_kv_heads][64 blocks] rows a second
- * launch joins.
+ * over pages; q and out [total_q][heads][D].  waves: per workgroup, 4 or 8, 16
+ * rows each.
+ * Prefill: blocks bounds the row blocks of the batch, sum over sequences of
+ * ceil(tokens * group / (16 waves)).  The keys of the longest are cut into
+ * chunks of at least min_tiles 32-key tiles, to about `budget` items per KV
+ * head and at most `items` (blocks + budget + 1); the parts [items][n_kv_heads]
+ * [16 waves] rows are joined by a second launch.  budget 0: not cut, items =
+ * blocks.
  * Decode: group i's members [group_start[i], group_start[i + 1]) share their
  * first prefix_len[i] positions, read once through the first member's table.
  * The keys are cut into about `budget` chunks per KV head, at most `items`,
@@ -410,7 +412,7 @@ typedef struct {
     float qscale;              /* softmax scale * log2(e) */
     const float *q;
     float *out;
-    int blocks, items, parts;
+    int waves, items, blocks;
     float *part_o, *part_ml;   /* D floats, and (max, sum), per row */
     int n_groups;
     const int *group_start, *prefix_len;

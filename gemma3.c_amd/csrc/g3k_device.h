@@ -31,6 +31,13 @@
     } while (0)
 #endif
 
+// Hides where a lane's value comes from, so that what is computed from it is
+// computed again in every pass of a loop instead of being kept in registers
+// across it (no instruction).
+#ifndef G3K_RECOMPUTE
+#define G3K_RECOMPUTE(x) asm volatile("" : "+v"(x))
+#endif
+
 // The XCD this wave runs on: the hardware register XCC_ID (gfx940 and
 // later), whose low 4 bits number the XCDs.  The host-emulation build
 // defines it as the workgroup id mod 8.

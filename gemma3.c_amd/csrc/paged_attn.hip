@@ -37,6 +37,8 @@
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
+#include <type_traits>
+
 #include "g3k.h"
 #include "g3k_device.h"
 #include "paged_body.h"
@@ -65,6 +67,11 @@ __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// Keeps the matrix operands' LDS reads and their MFMAs in the written order
+// (one step ahead), so that they take few registers; everything else moves
+// freely across.  Scheduler mask: VALU, SALU, vector memory, LDS writes.
+#define KEEP_OPERANDS() __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x10 | 0x20 | 0x40 | 0x200)
+
 __device__ __forceinline__ half2v cvt2(float a, float b) { return __builtin_convertvector((f32x2){a, b}, half2v); }
 
 // The power-of-two exponent of a block whose largest magnitude is m: m <
@@ -79,14 +86,15 @@ __device__ __forceinline__ int block_exponent(float m) {
 // x s as hi + lo, two values at a time.
 __device__ __forceinline__ void split2(float a, float b, float s, half2v &hi, half2v &lo) {
     hi = cvt2(a * s, b * s);
-    lo = cvt2(__builtin_fmaf(a, s, -(float)hi.x), __builtin_fmaf(b, s, -(float)hi.y));
+    lo.x = (_Float16)__builtin_fmaf(a, s, -(float)hi.x);
+    lo.y = (_Float16)__builtin_fmaf(b, s, -(float)hi.y);
 }
 
-// What a workgroup attends: query rows row0.. of a run of tokens over keys
-// [kbeg, kend) of table row b.
+// What a workgroup attends: the rows of a run of tokens over keys [kbeg, kend)
+// of table row b.
 struct Unit {
     int b, kbeg, kend;
-    int first, count;      // rows (of the group's heads): the first row's index among the run's, and how many
+    int count;             // rows (of the group's heads)
     int run;               // prefill: packed row of the run's first token; decode: the run's first sequence
     int pos;               // prefill: position of that token
 };
@@ -98,196 +106,206 @@ struct Lds {
     static constexpr int PL = BF16 ? 1 : 2;            // planes
     static constexpr int K_BYTES = 2 * 8 * PL * 1024;  // [key block][dim step][plane] operands
     static constexpr int V_BYTES = 16 * PL * 1024;     // [dim block][plane]
-    static constexpr int BUF = K_BYTES + V_BYTES;
-    static constexpr int BYTES = 2 * BUF;
+    static constexpr int BYTES = 2 * (K_BYTES + V_BYTES);
 };
 
-// One tile's rows in flight: this wave's 8 keys, 4 dims a lane.
-template <bool BF16>
-struct Raw;
-template <>
-struct Raw<false> {
-    f32x4 k[8], v[8];
-};
-template <>
-struct Raw<true> {
-    u32x2 k[8], v[8];
-};
-
-template <bool BF16>
-__device__ __forceinline__ void unpack(const Raw<BF16> &r, int i, bool v, float x[4]) {
-    if constexpr (BF16) {
-        const u32x2 u = v ? r.v[i] : r.k[i];
-        x[0] = __uint_as_float(u.x << 16);
-        x[1] = __uint_as_float(u.x & 0xffff0000u);
-        x[2] = __uint_as_float(u.y << 16);
-        x[3] = __uint_as_float(u.y & 0xffff0000u);
-    } else {
-        const f32x4 u = v ? r.v[i] : r.k[i];
-        x[0] = u.x;
-        x[1] = u.y;
-        x[2] = u.z;
-        x[3] = u.w;
-    }
-}
-
-// Where a tile's rows are: element offsets of this wave's 8 rows from the
-// head's first page row, and which of its two runs of 4 keys have no page.
-struct Place {
-    long long off[8];
-    int bad;
-};
-
-// Keys outside [kbeg, kend) take the nearest row inside, so nothing else is
-// read; their scores are masked.  A table entry outside the pool is never
-// followed: its run reads page 0 and is then zeroed and masked.
-__device__ __forceinline__ Place place_tile(const g3k_paged_args &a, const int *table, int tile, int wave, int kbeg,
-                                            int kend) {
-    Place p;
-    p.bad = 0;
-    const int j0 = tile * BK;
-    const int mask = (1 << a.s.page_shift) - 1;
-    if (j0 >= kbeg && j0 + BK <= kend) {
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int j = j0 + 16 * c + 4 * wave;
-            int page = __builtin_amdgcn_readfirstlane(table[j >> a.s.page_shift]);
-            if ((unsigned)page >= (unsigned)a.num_pages) {
-                page = 0;
-                p.bad |= 1 << c;
-            }
-            const long long o = page * a.page_stride + (long long)(j & mask) * D;
-#pragma unroll
-            for (int i = 0; i < 4; i++) p.off[4 * c + i] = o + i * D;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int j = clampi(j0 + 16 * (i >> 2) + 4 * wave + (i & 3), kbeg, kend - 1);
-            int page = __builtin_amdgcn_readfirstlane(table[j >> a.s.page_shift]);
-            if ((unsigned)page >= (unsigned)a.num_pages) {
-                page = 0;
-                p.bad |= 1 << (i >> 2);
-            }
-            p.off[i] = page * a.page_stride + (long long)(j & mask) * D;
-        }
-    }
-    return p;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void load_tile(const void *k, const void *v, const Place &p, int lane, Raw<BF16> &r) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
+// Rows of one matrix in flight: this wave's share of a tile's 32 keys, 4 dims
+// a lane.  Of NW waves, wave w brings lane group g = w % 4's keys: with 4 both
+// runs 4 g.. and 16 + 4 g.., with 8 the run 16 (w / 4) + 4 g...
+template <bool BF16, int NW>
+struct Raw {
+    static constexpr int RUNS = 8 / NW;
+    typename std::conditional<BF16, u32x2, f32x4>::type x[4 * RUNS];
+    __device__ __forceinline__ f32x4 get(int i) const {
         if constexpr (BF16) {
-            r.k[i] = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(k) + p.off[i] + 4 * lane);
+            const u32x2 u = x[i];
+            return (f32x4){__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u)};
         } else {
-            r.k[i] = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(k) + p.off[i] + 4 * lane);
+            return x[i];
         }
     }
+};
+
+__device__ const float zero_row[D] = {};
+
+// Where the rows of a walk are.  Looks pages up along it: 64 table entries in
+// a register, the next 64 on their way, so that a tile's lookup waits for no
+// memory.  A tile's entries never straddle two such runs (a tile is one
+// entry, or two from an even one).
+template <bool BF16, int NW>
+struct Finder {
+    static constexpr int RUNS = 8 / NW, ROW = D * (BF16 ? 2 : 4);
+    // Of a wave's share of a tile: byte offsets of its runs' first rows from
+    // the head's first page; whether all rows are between kbeg and kend, and
+    // which runs have no page.
+    struct Place {
+        long long off[RUNS];
+        int tile, bad;
+    };
+    const int *table;
+    int shift, mask, last, pages, kbeg, kend;     // last: entry of the walk
+    unsigned stride;                              // elements between pages
+    int base, now, next;
+
+    __device__ __forceinline__ void begin(const g3k_paged_args &a, const Unit &u, int lane) {
+        table = a.s.page_table + (long long)u.b * a.s.table_stride;
+        shift = a.s.page_shift;
+        mask = (1 << shift) - 1;
+        last = (u.kend - 1) >> shift;
+        pages = a.num_pages;
+        stride = (unsigned)a.page_stride;
+        kbeg = u.kbeg;
+        kend = u.kend;
+        base = (kbeg >> shift) & ~63;
+        now = table[clampi(base + lane, 0, last)];
+        next = table[clampi(base + 64 + lane, 0, last)];
+    }
+    __device__ __forceinline__ Place place(int tile, int wave, int lane) {
+        Place p;
+        p.tile = tile;
+        p.bad = 0;
+        const int j0 = tile * BK;
+        if ((j0 >> shift) >= base + 64) {
+            base += 64;
+            now = next;
+            next = table[clampi(base + 64 + lane, 0, last)];
+        }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if constexpr (BF16) {
-            r.v[i] = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(v) + p.off[i] + 4 * lane);
-        } else {
-            r.v[i] = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(v) + p.off[i] + 4 * lane);
+        for (int r = 0; r < RUNS; r++) {
+            const int j = j0 + 16 * (NW == 4 ? r : wave >> 2);
+            // (a run wholly outside the keys looks its nearest key's page up)
+            const int e = clampi(j, kbeg & ~15, kend - 1) >> shift;
+            const unsigned page = __builtin_amdgcn_readlane(now, e - base);
+            if (page >= (unsigned)pages) p.bad |= 1 << r;
+            p.off[r] = (long long)(((unsigned long long)page * stride + (unsigned)((j & mask) * D)) * (BF16 ? 2 : 4));
+        }
+        return p;
+    }
+    // Fetches the rows.  Keys outside [kbeg, kend) take the nearest row of
+    // their run inside, so nothing else is read; their scores are masked.  A
+    // page outside the pool is never followed, and neither is a run without a
+    // key: the rows are zeros.
+    __device__ __forceinline__ void fetch(const char *matrix, const Place &p, int wave, int lane, Raw<BF16, NW> &raw) const {
+        using T = typename std::conditional<BF16, u32x2, f32x4>::type;
+        const int j0 = p.tile * BK;
+        if (j0 >= kbeg && j0 + BK <= kend && !p.bad) {
+#pragma unroll
+            for (int r = 0; r < RUNS; r++) {
+                const char *row = matrix + p.off[r] + 4 * (wave & 3) * ROW;
+#pragma unroll
+                for (int i = 0; i < 4; i++) raw.x[4 * r + i] = *reinterpret_cast<const T *>(row + i * ROW + lane * (int)sizeof(T));
+            }
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < RUNS; r++) {
+            const int j = j0 + 16 * (NW == 4 ? r : wave >> 2);
+            const int lo = max(j, kbeg), hi = min(j + 16, kend) - 1;      // the run's keys
+            const bool none = lo > hi || ((p.bad >> r) & 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int k = clampi(j + 4 * (wave & 3) + i, lo, hi) - j;
+                const char *row = none ? reinterpret_cast<const char *>(zero_row) : matrix + p.off[r] + k * ROW;
+                raw.x[4 * r + i] = *reinterpret_cast<const T *>(row + lane * (int)sizeof(T));
+            }
         }
     }
+};
+
+// The largest magnitude of this lane's share of the rows in flight.
+template <bool BF16, int NW>
+__device__ __forceinline__ float rows_max(const Raw<BF16, NW> &raw) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4 * Raw<BF16, NW>::RUNS; i++) {
+        const f32x4 x = raw.get(i);
+        m = fmaxf(fmaxf(m, fabsf(x.x)), fabsf(x.y));
+        m = fmaxf(fmaxf(m, fabsf(x.z)), fabsf(x.w));
+    }
+    return m;
 }
 
-// Splits the rows in flight into operands and stores them, with the wave's
-// factors: {K's factor on the scores, the two runs' additive masks, V's
-// exponent}.
-template <bool BF16>
-__device__ __forceinline__ void store_tile(Raw<BF16> &r, int bad, char *buf, f32x4 *factors, int wave, int lane) {
+// K's rows (exponent e over the wave) as operands: lane holds dims 4 lane.. = half (lane & 1) of operand
+// lane group (lane >> 1) & 3 of dim step lane >> 3.  factors[run][group]: what
+// the scores of these keys are multiplied by, and their additive mask.
+template <bool BF16, int NW>
+__device__ __forceinline__ void store_k(const Raw<BF16, NW> &raw, int e, int bad, char *buf, f32x2 *factors, int wave, int lane) {
     using L = Lds<BF16>;
-    if (bad) {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if ((bad >> (i >> 2)) & 1) {
-                r.k[i] = 0;
-                r.v[i] = 0;
-            }
-    }
-    float mk = 0.f, mv = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float x[4];
-        unpack<BF16>(r, i, false, x);
-        mk = fmaxf(mk, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-        unpack<BF16>(r, i, true, x);
-        mv = fmaxf(mv, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-    }
-    const int ek = block_exponent(wave_max(mk)), ev = block_exponent(wave_max(mv));
-    const float sk = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ek), sv = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ev);
-    if (lane == 0)
-        factors[wave] = (f32x4){__builtin_amdgcn_ldexpf(1.0f, ek - X_EXP), bad & 1 ? -INFINITY : 0.f,
-                                bad & 2 ? -INFINITY : 0.f, __int_as_float(ev)};
-    // K: lane holds dims 4 lane.. = half (lane & 1) of operand lane group
-    // (lane >> 1) & 3 of dim step lane >> 3
+    const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
     char *kd = buf + (lane >> 3) * (L::PL * 1024) + ((lane >> 1) & 3) * 256 + (lane & 1) * 8;
     const int f = (lane >> 1) & 15;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float x[4];
-        unpack<BF16>(r, i, false, x);
-        char *d = kd + (i >> 2) * (8 * L::PL * 1024) + (((4 * wave + (i & 3)) ^ f) << 4);
-        half4v h, l;
-        if constexpr (BF16) {
-            h.xy = cvt2(x[0] * sk, x[1] * sk);
-            h.zw = cvt2(x[2] * sk, x[3] * sk);
-        } else {
-            half2v a, b;
-            split2(x[0], x[1], sk, a, b);
-            h.xy = a;
-            l.xy = b;
-            split2(x[2], x[3], sk, a, b);
-            h.zw = a;
-            l.zw = b;
-            *reinterpret_cast<half4v *>(d + 1024) = l;
-        }
-        *reinterpret_cast<half4v *>(d) = h;
-    }
-    // V: lane holds dims 4 lane + t of the 8 keys = operand lane lane & 15 of
-    // group `wave` of dim blocks 4 (lane >> 4) + t
-    char *vd = buf + L::K_BYTES + (lane >> 4) * (4 * L::PL * 1024) + wave * 256 + (lane & 15) * 16;
-    float x[8][4];
+    for (int r = 0; r < Raw<BF16, NW>::RUNS; r++) {
+        const int c = NW == 4 ? r : wave >> 2;
+        if (lane == 0) factors[4 * c + (wave & 3)] = (f32x2){__builtin_amdgcn_ldexpf(1.0f, e - X_EXP), (bad >> r) & 1 ? -INFINITY : 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; i++) unpack<BF16>(r, i, true, x[i]);
+        for (int i = 0; i < 4; i++) {
+            const f32x4 x = raw.get(4 * r + i);
+            char *d = kd + c * (8 * L::PL * 1024) + (((4 * (wave & 3) + i) ^ f) << 4);
+            half4v h, l;
+            if constexpr (BF16) {
+                h.xy = cvt2(x.x * sc, x.y * sc);
+                h.zw = cvt2(x.z * sc, x.w * sc);
+            } else {
+                half2v p, q;
+                split2(x.x, x.y, sc, p, q);
+                h.xy = p;
+                l.xy = q;
+                split2(x.z, x.w, sc, p, q);
+                h.zw = p;
+                l.zw = q;
+                *reinterpret_cast<half4v *>(d + 1024) = l;
+            }
+            *reinterpret_cast<half4v *>(d) = h;
+        }
+    }
+}
+
+// V's rows as operands: lane holds dims 4 lane + t of operand lane lane & 15 of
+// group g of dim blocks 4 (lane >> 4) + t, its keys 4 c.. of the operand's 8.
+template <bool BF16, int NW>
+__device__ __forceinline__ void store_v(const Raw<BF16, NW> &raw, int e, char *buf, int *exps, int wave, int lane) {
+    using L = Lds<BF16>;
+    constexpr int N = 4 * Raw<BF16, NW>::RUNS;
+    typedef _Float16 Keys __attribute__((ext_vector_type(N)));
+    const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
+    const int c = NW == 4 ? 0 : wave >> 2;
+    if (lane < 8 / NW) exps[4 * (NW == 4 ? lane : c) + (wave & 3)] = e;
+    char *vd = buf + (lane >> 4) * (4 * L::PL * 1024) + (wave & 3) * 256 + (lane & 15) * 16 + c * 8;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        half8 h, l;
+        Keys h, l;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
+        for (int i = 0; i < N; i += 2) {
+            const float x = raw.get(i)[t], y = raw.get(i + 1)[t];
             half2v hh, ll;
             if constexpr (BF16) {
-                hh = cvt2(x[i][t] * sv, x[i + 1][t] * sv);
+                hh = cvt2(x * sc, y * sc);
             } else {
-                split2(x[i][t], x[i + 1][t], sv, hh, ll);
+                split2(x, y, sc, hh, ll);
                 l[i] = ll.x;
                 l[i + 1] = ll.y;
             }
             h[i] = hh.x;
             h[i + 1] = hh.y;
         }
-        *reinterpret_cast<half8 *>(vd + t * (L::PL * 1024)) = h;
-        if constexpr (!BF16) *reinterpret_cast<half8 *>(vd + t * (L::PL * 1024) + 1024) = l;
+        *reinterpret_cast<Keys *>(vd + t * (L::PL * 1024)) = h;
+        if constexpr (!BF16) *reinterpret_cast<Keys *>(vd + t * (L::PL * 1024) + 1024) = l;
     }
 }
 
 // The rows of a wave: queries in registers, running softmax state, O^T.
-template <int MT>
 struct Rows {
-    half8 qh[MT][8], ql[MT][8];
-    f32x4 o[MT][16];
-    float factor[MT], m[MT], l[MT];   // l: this lane's keys only
-    int lo[MT], hi[MT];               // the keys this lane's row sees
-    int lo_min, lo_max, hi_min, hi_max;   // over the wave's rows
+    half8 qh[8], ql[8];
+    f32x4 o[16];
+    float factor, m, l;               // l: this lane's keys only
+    int lo, hi;                       // the keys this lane's row sees
+    int lo_max, hi_min;               // over the wave's rows: tiles between them need no mask
     int ev;                           // O^T's exponent: o = true o * 2^(X_EXP + P_EXP - ev), unnormalised
 };
 
-template <int MT>
-__device__ __forceinline__ void load_query(const float *q, bool live, float qscale, int mt, int lane, Rows<MT> &s) {
+__device__ __forceinline__ void load_query(const float *q, bool live, float qscale, int lane, Rows &s) {
     float x[8][8];
     float m = 0.f;
 #pragma unroll
@@ -305,207 +323,253 @@ __device__ __forceinline__ void load_query(const float *q, bool live, float qsca
     }
     const int e = block_exponent(col4_max(m));
     const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
-    s.factor[mt] = __builtin_amdgcn_ldexpf(qscale, e - X_EXP);
+    s.factor = __builtin_amdgcn_ldexpf(qscale, e - X_EXP);
 #pragma unroll
     for (int kk = 0; kk < 8; kk++)
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             half2v h, l;
             split2(x[kk][i], x[kk][i + 1], sc, h, l);
-            s.qh[mt][kk][i] = h.x;
-            s.qh[mt][kk][i + 1] = h.y;
-            s.ql[mt][kk][i] = l.x;
-            s.ql[mt][kk][i + 1] = l.y;
+            s.qh[kk][i] = h.x;
+            s.qh[kk][i + 1] = h.y;
+            s.ql[kk][i] = l.x;
+            s.ql[kk][i + 1] = l.y;
         }
 }
 
-// One tile's keys for the wave's rows.
-template <bool BF16, int MT>
-__device__ __forceinline__ void attend_tile(const char *buf, const f32x4 *factors, int tile, int lane, Rows<MT> &s) {
+// S^T of a tile.
+template <bool BF16>
+__device__ __forceinline__ void tile_scores(const char *buf, int lane, const Rows &s, f32x4 (&sc)[2]) {
     using L = Lds<BF16>;
-    const int j0 = tile * BK;
     const int g = lane >> 4, c = lane & 15;
-    f32x4 sc[MT][2];
+    f32x4 sx[2];                  // the products with a lo plane: four sums, so that
+    sc[0] = sc[1] = sx[0] = sx[1] = (f32x4){0.f, 0.f, 0.f, 0.f};   // none waits for its last MFMA
+    half8 kh[2][2], kl[2][2];     // operands of this dim step and the next
+    const auto read = [&](int kk) {
+        const char *kp = buf + kk * (L::PL * 1024) + g * 256 + ((c ^ ((4 * kk + g) & 15)) << 4);
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) sc[mt][0] = sc[mt][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int kt = 0; kt < 2; kt++) {
+            kh[kk & 1][kt] = *reinterpret_cast<const half8 *>(kp + kt * (8 * L::PL * 1024));
+            if constexpr (!BF16) kl[kk & 1][kt] = *reinterpret_cast<const half8 *>(kp + kt * (8 * L::PL * 1024) + 1024);
+        }
+    };
+    read(0);
 #pragma unroll
     for (int kk = 0; kk < 8; kk++) {
-        const char *kp = buf + kk * (L::PL * 1024) + g * 256 + ((c ^ ((4 * kk + g) & 15)) << 4);
-        half8 kh[2], kl[2];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            kh[kt] = *reinterpret_cast<const half8 *>(kp + kt * (8 * L::PL * 1024));
-            if constexpr (!BF16) kl[kt] = *reinterpret_cast<const half8 *>(kp + kt * (8 * L::PL * 1024) + 1024);
-        }
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) sc[mt][kt] = mfma(kh[kt], s.qh[mt][kk], sc[mt][kt]);
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) sc[mt][kt] = mfma(kh[kt], s.ql[mt][kk], sc[mt][kt]);
+        const int x = kk & 1;
+        if (kk < 7) read(kk + 1);
+        sc[0] = mfma(kh[x][0], s.qh[kk], sc[0]);
+        sx[0] = mfma(kh[x][0], s.ql[kk], sx[0]);
+        sx[1] = mfma(kh[x][1], s.ql[kk], sx[1]);
+        sc[1] = mfma(kh[x][1], s.qh[kk], sc[1]);
         if constexpr (!BF16) {
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) sc[mt][kt] = mfma(kl[kt], s.qh[mt][kk], sc[mt][kt]);
+            sx[0] = mfma(kl[x][0], s.qh[kk], sx[0]);
+            sx[1] = mfma(kl[x][1], s.qh[kk], sx[1]);
         }
+        KEEP_OPERANDS();
     }
-    const f32x4 fac = factors[g];
-    const int ev = __float_as_int(fac.w);
-    // the tile's V exponent, over the four lane groups
-    const int ev_tile = max(max(__float_as_int(factors[0].w), __float_as_int(factors[1].w)),
-                            max(__float_as_int(factors[2].w), __float_as_int(factors[3].w)));
+    sc[0] += sx[0];
+    sc[1] += sx[1];
+}
+
+// Scores to probabilities (in place), the running max and sum, and O^T's
+// rescaling, which is rare: a row's max moves only when a score outgrows it by
+// 2^LAZY.  fac[run]: the factor and mask of this lane group's keys.
+__device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, int lane, Rows &s, f32x4 (&sc)[2]) {
+    const int j0 = tile * BK, g = lane >> 4;
     const bool ragged = j0 < s.lo_max || j0 + BK > s.hi_min;
-    float tmax[MT];
-    bool grow = ev_tile > s.ev;
+    float t = M_NONE;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const float f = s.factor[mt] * fac.x;
-        float t = M_NONE;
+    for (int kt = 0; kt < 2; kt++) {
+        const float f = s.factor * fac[kt].x;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            const float bias = kt ? fac.z : fac.y;
+        for (int r = 0; r < 4; r++) sc[kt][r] = __builtin_fmaf(sc[kt][r], f, fac[kt].y);
+    }
+    if (ragged) {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float x = __builtin_fmaf(sc[mt][kt][r], f, bias);
-                if (ragged) {
-                    const int j = j0 + 16 * kt + 4 * g + r;
-                    if (j < s.lo[mt] || j >= s.hi[mt]) x = -INFINITY;
-                }
-                sc[mt][kt][r] = x;
-                t = fmaxf(t, x);
-            }
-        }
-        tmax[mt] = col4_max(t);
-        grow |= tmax[mt] > s.m[mt] + LAZY;
-    }
-    // O^T and l are rescaled when a row's max outgrows its reference by
-    // 2^LAZY, or V's exponent the one O^T is held at (two bits above what it
-    // was first, so ordinary tiles do not move it)
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-        const int e = ev_tile > s.ev ? ev_tile + 2 : s.ev;
-        const float down = s.ev == E_NONE ? 0.f : __builtin_amdgcn_ldexpf(1.0f, s.ev - e);
-        s.ev = e;
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            const float m = tmax[mt] > s.m[mt] + LAZY ? tmax[mt] : s.m[mt];
-            const float keep = fast_exp2(s.m[mt] - m);
-            s.m[mt] = m;
-            s.l[mt] *= keep;
-            const float x = keep * down;
-#pragma unroll
-            for (int d = 0; d < 16; d++) s.o[mt][d] *= x;
-        }
-    }
-    const float pf = __builtin_amdgcn_ldexpf(1.0f, P_EXP + ev - s.ev);
-    half8 ph[MT], pl[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int r = 0; r < 4; r += 2) {
-                const float a = fast_exp2(sc[mt][kt][r] - s.m[mt]), b = fast_exp2(sc[mt][kt][r + 1] - s.m[mt]);
-                s.l[mt] += a + b;
-                half2v h, l;
-                split2(a, b, pf, h, l);
-                ph[mt][4 * kt + r] = h.x;
-                ph[mt][4 * kt + r + 1] = h.y;
-                pl[mt][4 * kt + r] = l.x;
-                pl[mt][4 * kt + r + 1] = l.y;
+                const int j = j0 + 16 * kt + 4 * g + r;
+                if (j < s.lo || j >= s.hi) sc[kt][r] = -INFINITY;
             }
     }
-    const char *vp = buf + L::K_BYTES + lane * 16;
 #pragma unroll
-    for (int d = 0; d < 16; d++) {
-        const half8 vh = *reinterpret_cast<const half8 *>(vp + d * (L::PL * 1024));
+    for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) s.o[mt][d] = mfma(vh, ph[mt], s.o[mt][d]);
+        for (int r = 0; r < 4; r++) t = fmaxf(t, sc[kt][r]);
+    t = col4_max(t);
+    const bool up = t > s.m + LAZY;
+    if (__builtin_amdgcn_ballot_w64(up)) {
+        const float m = up ? t : s.m;
+        const float keep = fast_exp2(s.m - m);
+        s.m = m;
+        s.l *= keep;
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) s.o[mt][d] = mfma(vh, pl[mt], s.o[mt][d]);
-        if constexpr (!BF16) {
-            const half8 vl = *reinterpret_cast<const half8 *>(vp + d * (L::PL * 1024) + 1024);
+        for (int d = 0; d < 16; d++) s.o[d] *= keep;
+    }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) s.o[mt][d] = mfma(vl, ph[mt], s.o[mt][d]);
+    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            sc[kt][r] = fast_exp2(sc[kt][r] - s.m);
+            s.l += sc[kt][r];
+        }
+}
+
+// P as the operand of P.V, scaled by its keys' V exponent against O^T's.  The
+// one O^T is held at is two bits above what the first tile has, so ordinary
+// tiles do not move it.
+__device__ __forceinline__ void split_p(const f32x4 (&p)[2], const int *exps, int lane, Rows &s, half8 &ph, half8 &pl) {
+    int most = exps[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) most = max(most, exps[i]);
+    const int top = __builtin_amdgcn_readfirstlane(most);
+    if (top > s.ev) {
+        const float down = s.ev == E_NONE ? 0.f : __builtin_amdgcn_ldexpf(1.0f, s.ev - top - 2);
+        s.ev = top + 2;
+#pragma unroll
+        for (int d = 0; d < 16; d++) s.o[d] *= down;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) {
+        const float f = __builtin_amdgcn_ldexpf(1.0f, P_EXP + exps[4 * kt + (lane >> 4)] - s.ev);
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            half2v h, l;
+            split2(p[kt][r], p[kt][r + 1], f, h, l);
+            ph[4 * kt + r] = h.x;
+            ph[4 * kt + r + 1] = h.y;
+            pl[4 * kt + r] = l.x;
+            pl[4 * kt + r + 1] = l.y;
         }
     }
 }
 
-// The whole walk of a workgroup over its unit's tiles.  Tile t + 1 is split
-// and stored while tile t + 2 is fetched, then tile t is attended: one
-// barrier a tile, and a fetch has a whole tile's work to arrive.
-template <bool BF16, int MT>
-__device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Unit &u, char *lds, f32x4 *factors, int wave,
-                                     int lane, Rows<MT> &s) {
+// O^T += V^T P^T of a tile.
+template <bool BF16>
+__device__ __forceinline__ void tile_values(const char *buf, int lane, half8 ph, half8 pl, Rows &s) {
     using L = Lds<BF16>;
-    const int t0 = u.kbeg / BK, t1 = u.kend > u.kbeg ? (u.kend + BK - 1) / BK : t0;
-    if (t0 >= t1) return;
-    const int *table = a.s.page_table + (long long)u.b * a.s.table_stride;
-    const long long head_off = ((long long)head << a.s.page_shift) * D;
-    const size_t es = BF16 ? 2 : 4;
-    const void *kb = static_cast<const char *>(a.k) + head_off * es, *vb = static_cast<const char *>(a.v) + head_off * es;
-    Raw<BF16> raw;
-    Place p = place_tile(a, table, t0, wave, u.kbeg, u.kend);
-    load_tile<BF16>(kb, vb, p, lane, raw);
-    int bad = p.bad;
-    store_tile<BF16>(raw, bad, lds, factors, wave, lane);
-    if (t0 + 1 < t1) {
-        p = place_tile(a, table, t0 + 1, wave, u.kbeg, u.kend);
-        load_tile<BF16>(kb, vb, p, lane, raw);
-        bad = p.bad;
+    const char *vp = buf + lane * 16;
+    // a step takes hi.hi of one dim block, hi.lo of the last and lo.hi of the
+    // one before: no sum waits for its last MFMA
+    half8 vh[4], vl[3];
+    const auto read_hi = [&](int d) { vh[d & 3] = *reinterpret_cast<const half8 *>(vp + d * (L::PL * 1024)); };
+    read_hi(0);
+    read_hi(1);
+#pragma unroll
+    for (int d = 0; d < 18; d++) {
+        if (d < 14) read_hi(d + 2);
+        if constexpr (!BF16) {
+            if (d < 16) vl[d % 3] = *reinterpret_cast<const half8 *>(vp + d * (L::PL * 1024) + 1024);
+        }
+        if (d < 16) s.o[d] = mfma(vh[d & 3], ph, s.o[d]);
+        if (d > 0 && d < 17) s.o[d - 1] = mfma(vh[(d - 1) & 3], pl, s.o[d - 1]);
+        if constexpr (!BF16) {
+            if (d > 1) s.o[d - 2] = mfma(vl[(d - 2) % 3], ph, s.o[d - 2]);
+        }
+        KEEP_OPERANDS();
+    }
+}
+
+// The walk of a workgroup over its unit's tiles, counted from 0 here.  A step
+// is a phase on the matrix units, M(i): scores of tile i + 1, values of tile
+// i; and one on the vector units, V(i): softmax of tile i + 1, this wave's
+// rows of later tiles split and stored (and the next ones fetched).  With 8
+// waves, waves w and w + 4 share a SIMD; the second four run one phase later,
+// so that one is in M while the other is in V, and store one tile further
+// ahead (`lead`).  Tile i + 2 of K goes where tile i was, i + 1 of V where i - 1
+// was, both at least a phase after their last read and before their first;
+// what V(i) needs of the factors is read in M(i), before others write them.
+template <bool BF16, int NW>
+__device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Unit &u, char *lds, f32x2 *factors, int *exps, int wave,
+                                     int lane, Rows &s) {
+    using L = Lds<BF16>;
+    const int t0 = u.kbeg / BK, n = u.kend > u.kbeg ? (u.kend + BK - 1) / BK - t0 : 0;
+    if (n <= 0) return;
+    char *kbuf = lds, *vbuf = lds + 2 * L::K_BYTES;
+    const long long head_off = ((long long)head << a.s.page_shift) * D * (BF16 ? 2 : 4);
+    const char *kb = static_cast<const char *>(a.k) + head_off, *vb = static_cast<const char *>(a.v) + head_off;
+    Finder<BF16, NW> find;
+    find.begin(a, u, lane);
+    Raw<BF16, NW> rk, rv;
+    int ik = 0, iv = 0;       // tiles in flight; past the end, the last one again
+    auto pk = find.place(t0, wave, lane), pv = pk;
+    find.fetch(kb, pk, wave, lane, rk);
+    find.fetch(vb, pv, wave, lane, rv);
+    // K's next tile has been looked up when V's is fetched
+    const auto next_k = [&](int e) {
+        store_k<BF16, NW>(rk, e, pk.bad, kbuf + (ik & 1) * L::K_BYTES, factors + 8 * (ik & 1), wave, lane);
+        ik++;
+        pv = pk;
+        pk = find.place(t0 + min(ik, n - 1), wave, lane);
+        find.fetch(kb, pk, wave, lane, rk);
+    };
+    const auto next_v = [&](int e) {
+        store_v<BF16, NW>(rv, e, vbuf + (iv & 1) * L::V_BYTES, exps + 8 * (iv & 1), wave, lane);
+        iv++;
+        find.fetch(vb, pv, wave, lane, rv);
+    };
+    const int lead = NW == 8 ? wave >> 2 : 0;
+    const auto exponent = [&](const Raw<BF16, NW> &r) { return block_exponent(wave_max(rows_max<BF16, NW>(r))); };
+    next_k(exponent(rk));
+    if (lead) {
+        pv = pk;
+        next_v(exponent(rv));
+        next_k(exponent(rk));
     }
     // only LDS has to have arrived at these barriers: 63 vector memory
     // operations may stay in flight
     G3K_WAIT_BARRIER(63);
-    for (int t = t0; t < t1; t++) {
-        const int x = (t - t0) & 1;
-        if (t + 1 < t1) {
-            store_tile<BF16>(raw, bad, lds + (x ^ 1) * L::BUF, factors + 4 * (x ^ 1), wave, lane);
-            if (t + 2 < t1) {
-                p = place_tile(a, table, t + 2, wave, u.kbeg, u.kend);
-                load_tile<BF16>(kb, vb, p, lane, raw);
-                bad = p.bad;
-            }
+    if (lead) G3K_WAIT_BARRIER(63);
+    f32x4 p[2];             // tile i's scores, then probabilities
+    half8 ph, pl;
+    for (int i = 0; i < n; i++) {
+        const int t = t0 + i, x = i & 1;
+        G3K_RECOMPUTE(lane);
+        // M(i - 1)
+        f32x4 sc[2];
+        const f32x2 *f = factors + 8 * x + (lane >> 4);
+        const f32x2 fac[2] = {f[0], f[4]};
+        tile_scores<BF16>(kbuf + x * L::K_BYTES, lane, s, sc);
+        if (i > 0) {
+            split_p(p, exps + 8 * (x ^ 1), lane, s, ph, pl);
+            tile_values<BF16>(vbuf + (x ^ 1) * L::V_BYTES, lane, ph, pl, s);
         }
-        if (t * BK < s.hi_max && t * BK + BK > s.lo_min)
-            attend_tile<BF16, MT>(lds + x * L::BUF, factors + 4 * x, t, lane, s);
+        p[0] = sc[0];
+        p[1] = sc[1];
+        if (NW == 8) G3K_WAIT_BARRIER(63);
+        // V(i - 1)
+        // (three chains of cross-lane steps side by side)
+        const int ek = exponent(rk), ev = exponent(rv);
+        tile_softmax(fac, t, lane, s, p);
+        next_k(ek);
+        next_v(ev);
         G3K_WAIT_BARRIER(63);
     }
+    split_p(p, exps + 8 * ((n - 1) & 1), lane, s, ph, pl);
+    tile_values<BF16>(vbuf + ((n - 1) & 1) * L::V_BYTES, lane, ph, pl, s);
+    // the second four are a phase behind: one barrier more before, one less after
+    if (NW == 8 && !lead) G3K_WAIT_BARRIER(63);
 }
 
 // Row state before the walk, from the keys each lane's row sees: [lo, hi),
 // or [0, INT_MAX) for a lane without a row.
-template <int MT>
-__device__ __forceinline__ void begin_rows(Rows<MT> &s) {
-    int lo_min = INT_MAX, hi_max = 0, lo_max = 0, hi_min = INT_MAX;
+__device__ __forceinline__ void begin_rows(Rows &s) {
+    s.m = M_NONE;
+    s.l = 0.f;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        s.m[mt] = M_NONE;
-        s.l[mt] = 0.f;
-#pragma unroll
-        for (int d = 0; d < 16; d++) s.o[mt][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (s.hi[mt] == INT_MAX) continue;      // not a row
-        if (s.hi[mt] > s.lo[mt]) {
-            lo_min = min(lo_min, s.lo[mt]);
-            hi_max = max(hi_max, s.hi[mt]);
-        }
-        lo_max = max(lo_max, s.lo[mt]);
-        hi_min = min(hi_min, s.hi[mt]);
-    }
+    for (int d = 0; d < 16; d++) s.o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     s.ev = E_NONE;
-    s.lo_min = __builtin_amdgcn_readfirstlane(row16_min_int(lo_min));
-    s.hi_max = -__builtin_amdgcn_readfirstlane(row16_min_int(-hi_max));
-    s.lo_max = -__builtin_amdgcn_readfirstlane(row16_min_int(-lo_max));
-    s.hi_min = __builtin_amdgcn_readfirstlane(row16_min_int(hi_min));
+    const bool row = s.hi != INT_MAX;
+    s.lo_max = -__builtin_amdgcn_readfirstlane(row16_min_int(row ? -s.lo : 0));
+    s.hi_min = __builtin_amdgcn_readfirstlane(row16_min_int(row ? s.hi : INT_MAX));
 }
 
-// Stores this lane's share of row mt: the normalised output, and for a part
-// its (max, sum).
-template <int MT>
-__device__ __forceinline__ void store_row(const Rows<MT> &s, int mt, float *out, float *ml, int lane) {
-    const float l = col4_sum(s.l[mt]);
+// Stores this lane's share of its row (if it has one): the normalised output,
+// and for a part its (max, sum).
+__device__ __forceinline__ void store_row(const Rows &s, float *out, float *ml, int lane) {
+    const float l = col4_sum(s.l);
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
     const int e = s.ev == E_NONE ? 0 : s.ev - X_EXP - P_EXP;
     if (!out) return;
@@ -515,107 +579,171 @@ __device__ __forceinline__ void store_row(const Rows<MT> &s, int mt, float *out,
         for (int r = 0; r < 4; r++) {
             f32x4 x;
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = __builtin_amdgcn_ldexpf(s.o[mt][4 * T + t][r] * inv, e);
+            for (int t = 0; t < 4; t++) x[t] = __builtin_amdgcn_ldexpf(s.o[4 * T + t][r] * inv, e);
             *reinterpret_cast<f32x4 *>(out + 64 * T + 16 * (lane >> 4) + 4 * r) = x;
         }
     if (ml && lane < 16) {
-        ml[0] = s.m[mt];
+        ml[0] = s.m;
         ml[1] = l;
     }
 }
 
 // ---- packed prompts ------------------------------------------------------------
 
-// Row blocks of a sequence of n tokens.
-__device__ __forceinline__ int row_blocks(const g3k_paged_args &a, int n, int rows) {
-    const int t = rows / a.group;   // tokens per block
-    return (n + t - 1) / t;
+// A sequence's new tokens as blocks of T tokens (ROWS rows of a head group).
+struct Prompt {
+    int first, n, pos, blocks;     // packed row, tokens, position of the first, blocks
+    bool all;                      // no block's window leaves keys out
+    __device__ __forceinline__ int kend(int rb, int T) const {
+        const int e = pos + min((rb + 1) * T, n);
+        return e > 0 ? e : 0;
+    }
+    // tiles of the block with the most, or (behind a window) at most that many
+    __device__ __forceinline__ int most_tiles(const g3k_paged_args &a, int T) const {
+        const int whole = (max(pos + n, 0) + BK - 1) / BK;
+        return all ? whole : min(whole, (a.window + T) / BK + 2);
+    }
+    // the first block with more than p chunks of c tiles (or an earlier one,
+    // behind a window): a block's keys end with it
+    __device__ __forceinline__ int first_with(int p, int c, int T) const {
+        const int x = p * c * BK - pos;
+        return p == 0 || !all || x < 0 ? 0 : min(x / T, blocks);
+    }
+    __device__ __forceinline__ int chunks(const g3k_paged_args &a, int c, int T) const {
+        const int t = most_tiles(a, T);
+        return t > 0 ? (t + c - 1) / c : 1;
+    }
+    __device__ __forceinline__ int items(const g3k_paged_args &a, int c, int T) const {
+        const int k = chunks(a, c, T);
+        if (!all || k == 1) return blocks * k;
+        int sum = 0;
+        for (int p = 0; p < k; p++) sum += blocks - first_with(p, c, T);
+        return sum;
+    }
+};
+
+__device__ __forceinline__ Prompt prompt_of(const g3k_paged_args &a, int b, int T) {
+    Prompt p = {0, 0, 0, 0, true};
+    if (b >= a.s.num_seqs) return p;
+    seq_rows(a.s, b, p.first, p.n);
+    const int len = seq_len(a.s, b);
+    p.pos = len - p.n;
+    p.blocks = (p.n + T - 1) / T;
+    p.all = a.window >= len;
+    return p;
 }
 
-// Block `blk` of the batch: its sequence and rows, the last block of each
-// sequence first (the one with the most keys).  False past the last block.
-__device__ bool find_block(const g3k_paged_args &a, int blk, int rows, int lane, Unit &u) {
+constexpr int MAX_TILES = G3K_PAGED_MAX_LEN / BK;
+
+// Tiles per chunk: the longest blocks' keys are cut so that the batch is about
+// a.budget items per KV head, whatever the lengths.  Every wave adds the
+// lengths up for itself (a causal block has keys up to its last token).
+// Without a budget nothing is cut.
+__device__ int prompt_chunk(const g3k_paged_args &a, int T, int lane) {
+    if (a.budget <= 0) return MAX_TILES;
+    float total = 0.f;      // an upper estimate
+    for (int base = 0; base < a.s.num_seqs; base += 64) {
+        const Prompt p = prompt_of(a, base + lane, T);
+        float t = 0.f;
+        if (p.blocks > 0) {
+            const float n = (float)p.blocks;
+            t = p.all ? n * ((float)max(p.pos, 0) * (1.0f / BK) + 1.0f) + 0.5f * n * (n + 1.0f) * (float)T * (1.0f / BK)
+                      : n * (float)p.most_tiles(a, T);
+        }
+        total += wave_sum(t);
+    }
+    const float c = total * 1.0001f / (float)a.budget + 1.0f;
+    return c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
+}
+
+// What a workgroup of the packed kernel does: a block's rows, over its keys.
+__device__ __forceinline__ void set_block(const g3k_paged_args &a, int b, const Prompt &p, int rb, int T, Unit &u) {
+    const int tok = rb * T, left = min(p.n - tok, T);
+    u.b = b;
+    u.run = p.first + tok;
+    u.pos = p.pos + tok;
+    u.count = left * a.group;
+    u.kend = max(u.pos + left, 0);
+    u.kbeg = max(u.pos + 1 - a.window, 0);
+}
+__device__ __forceinline__ int block_chunks(const Unit &u, int c) {
+    const int n = u.kend > u.kbeg ? (u.kend + BK - 1) / BK - u.kbeg / BK : 0;
+    return n > 0 ? (n + c - 1) / c : 1;
+}
+__device__ __forceinline__ Prompt uniform(const Prompt &p, int lane) {
+    Prompt r;
+    r.first = __builtin_amdgcn_readlane(p.first, lane);
+    r.n = __builtin_amdgcn_readlane(p.n, lane);
+    r.pos = __builtin_amdgcn_readlane(p.pos, lane);
+    r.blocks = __builtin_amdgcn_readlane(p.blocks, lane);
+    r.all = __builtin_amdgcn_readlane((int)p.all, lane) != 0;
+    return r;
+}
+
+// Item `item` of the batch: chunk by chunk of each sequence, its last block
+// (the one with the most keys) first.  False past the last item.
+__device__ bool find_item(const g3k_paged_args &a, int item, int c, int T, int lane, Unit &u, int &chunk) {
     int before = 0;
     for (int base = 0; base < a.s.num_seqs; base += 64) {
-        int first = 0, n = 0;
-        if (base + lane < a.s.num_seqs) seq_rows(a.s, base + lane, first, n);
-        const int nb = row_blocks(a, n, rows);
-        const int upto = wave_scan_int(nb, lane);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(blk - before < upto);
+        const Prompt mine = prompt_of(a, base + lane, T);
+        const int n = mine.blocks > 0 ? mine.items(a, c, T) : 0;
+        const int upto = wave_scan_int(n, lane);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(item - before < upto);
         if (past) {
             const int at = __builtin_ctzll(past);
-            const int b = base + at;
-            const int rb = __shfl(upto, at) - 1 - (blk - before);
-            n = __builtin_amdgcn_readfirstlane(__shfl(n, at));
-            first = __builtin_amdgcn_readfirstlane(__shfl(first, at));
-            const int t = rows / a.group;
-            const int tok = __builtin_amdgcn_readfirstlane(rb) * t;
-            const int left = n - tok < t ? n - tok : t;
-            const int len = __builtin_amdgcn_readfirstlane(seq_len(a.s, b));
-            u.b = b;
-            u.run = first + tok;
-            u.pos = len - n + tok;
-            u.first = 0;
-            u.count = left * a.group;
-            u.kend = u.pos + left > 0 ? u.pos + left : 0;
-            u.kbeg = u.pos + 1 - a.window > 0 ? u.pos + 1 - a.window : 0;
+            const Prompt p = uniform(mine, at);
+            int k = item - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+            for (chunk = 0;; chunk++) {
+                const int here = p.blocks - p.first_with(chunk, c, T);
+                if (k < here) break;
+                k -= here;
+            }
+            set_block(a, base + at, p, p.blocks - 1 - k, T, u);
             return true;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
 
-// Parts of a block's keys: at least PART_TILES tiles each, at most `most`.
-constexpr int PART_TILES = 8;
-__device__ __forceinline__ int split_keys(const Unit &u, int most, int part, int &kbeg, int &kend) {
-    const int t0 = u.kbeg / BK, n = u.kend > u.kbeg ? (u.kend + BK - 1) / BK - t0 : 0;
-    int parts = n / PART_TILES < most ? n / PART_TILES : most;
-    if (parts < 1) parts = 1;
-    const int per = (n + parts - 1) / parts;
-    parts = per > 0 ? (n + per - 1) / per : 1;
-    const int b = (t0 + part * per) * BK, e = (t0 + part * per + per) * BK;
-    kbeg = b > u.kbeg ? b : u.kbeg;
-    kend = e < u.kend ? e : u.kend;
-    return parts;
-}
-
-template <bool BF16, int MT>
-__global__ __launch_bounds__(256, 1) void paged_prefill_kernel(g3k_paged_args a) {
+template <bool BF16, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void paged_prefill_kernel(g3k_paged_args a) {
     __shared__ __align__(16) char lds[Lds<BF16>::BYTES];
-    __shared__ f32x4 factors[8];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ f32x2 factors[16];
+    __shared__ int exps[16];
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.n_kv_heads, item = blockIdx.x / a.n_kv_heads;
-    const int part = item % a.parts, blk = item / a.parts;
-    constexpr int ROWS = 64 * MT;
+    constexpr int ROWS = 16 * NW;
     Unit u;
-    if (!find_block(a, blk, ROWS, lane, u)) return;
-    int kbeg, kend;
-    const int parts = split_keys(u, a.parts, part, kbeg, kend);
-    if (part >= parts) return;
-    Rows<MT> s;
+    int chunk;
+    const int T = ROWS / a.group, c = __builtin_amdgcn_readfirstlane(prompt_chunk(a, T, lane));
+    if (!find_item(a, item, c, T, lane, u, chunk)) return;
+    const int parts = block_chunks(u, c);
+    if (chunk >= parts) return;
+    const int kbeg = max(u.kbeg, (u.kbeg / BK + chunk * c) * BK), kend = min((long long)u.kend, (u.kbeg / BK + (chunk + 1LL) * c) * BK);
+    Rows s;
     const int gs = __builtin_ctz(a.group);
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int row = (wave * MT + mt) * 16 + (lane & 15);
+    {
+        const int row = wave * 16 + (lane & 15);
         const bool live = row < u.count;
         const int tok = row >> gs, h = head * a.group + (row & (a.group - 1));
         const int hi = u.pos + tok + 1;
-        s.hi[mt] = live ? min(hi, kend) : INT_MAX;
-        s.lo[mt] = live ? max(hi - a.window, kbeg) : 0;
-        load_query<MT>(a.q + ((long long)(u.run + tok) * a.n_kv_heads * a.group + h) * D, live, a.qscale, mt, lane, s);
+        s.hi = live ? min(hi, kend) : INT_MAX;
+        s.lo = live ? max(hi - a.window, kbeg) : 0;
+        load_query(a.q + ((long long)(u.run + tok) * a.n_kv_heads * a.group + h) * D, live, a.qscale, lane, s);
     }
-    begin_rows<MT>(s);
+    begin_rows(s);
     u.kbeg = kbeg;
     u.kend = kend;
-    walk<BF16, MT>(a, head, u, lds, factors, wave, lane, s);
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int row = (wave * MT + mt) * 16 + (lane & 15);
+    walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, s);
+    G3K_RECOMPUTE(lane);      // no output address is kept through the walk
+    {
+        const int row = wave * 16 + (lane & 15);
         float *out = nullptr, *ml = nullptr;
         if (row < u.count) {
             if (parts > 1) {
-                const long long slot = ((long long)(blk * a.parts + part) * a.n_kv_heads + head) * ROWS + row;
+                const long long slot = ((long long)item * a.n_kv_heads + head) * ROWS + row;
                 out = a.part_o + slot * D;
                 ml = a.part_ml + slot * 2;
             } else {
@@ -623,60 +751,93 @@ __global__ __launch_bounds__(256, 1) void paged_prefill_kernel(g3k_paged_args a)
                                (row & (a.group - 1))) * D;
             }
         }
-        store_row<MT>(s, mt, out, ml, lane);
+        store_row(s, out, ml, lane);
     }
 }
 
-// Sums n parts of a row, part i at o + i * stride rows; every lane 4 dims.
-// n <= 64; the statistics are one load a lane.
+// A row's parts joined; every lane 4 dims.
 struct Joined {
     f32x4 o;
     float m, l;
-};
-__device__ __forceinline__ void join_parts(const float *o, const float *ml, long long stride, int n, int lane, Joined &j) {
-    for (int base = 0; base < n; base += 64) {
-        const int k = n - base < 64 ? n - base : 64;
-        float m = M_NONE, l = 0.f;
-        if (lane < k) {
-            const float *p = ml + (base + lane) * stride * 2;
-            m = p[0];
-            l = p[1];
+    __device__ __forceinline__ void clear() {
+        o = (f32x4){0.f, 0.f, 0.f, 0.f};
+        m = M_NONE;
+        l = 0.f;
+    }
+    // Adds n <= 64 parts: lane i's slot is part i's row.  The statistics are
+    // one load a lane.
+    __device__ __forceinline__ void add(const g3k_paged_args &a, long long slot, int n, int lane) {
+        float pm = M_NONE, pl = 0.f;
+        if (lane < n) {
+            pm = a.part_ml[2 * slot];
+            pl = a.part_ml[2 * slot + 1];
         }
-        const float top = fmaxf(wave_max(m), j.m);
-        const float w = l * fast_exp2(m - top);
-        const float keep = fast_exp2(j.m - top);
-        j.o *= keep;
-        j.l = j.l * keep + wave_sum(w);
-        j.m = top;
-        for (int i = 0; i < k; i++) {
-            const float wi = __shfl(w, i);
-            // a part without a visible key has no say, whatever its output
-            if (wi != 0.f) j.o += wi * *reinterpret_cast<const f32x4 *>(o + (base + i) * stride * D + 4 * lane);
+        const float top = fmaxf(wave_max(pm), m);
+        const float w = pl * fast_exp2(pm - top), keep = fast_exp2(m - top);
+        o *= keep;
+        l = l * keep + wave_sum(w);
+        m = top;
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
+            const long long si = (long long)(unsigned)__builtin_amdgcn_readlane((int)slot, i) |
+                                 (long long)__builtin_amdgcn_readlane((int)(slot >> 32), i) << 32;
+            o += wi * *reinterpret_cast<const f32x4 *>(a.part_o + si * D + 4 * lane);
         }
     }
-}
+    __device__ __forceinline__ void store(float *out, int lane) const {
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+        *reinterpret_cast<f32x4 *>(out + 4 * lane) = o * inv;
+    }
+};
 
-// One wave per row of a block whose keys were split.
-template <int MT>
+// MERGE_ROWS rows of a block and head per workgroup, one wave a row.  Blocks
+// of one chunk were stored whole.
+constexpr int MERGE_ROWS = 8;
+template <int NW>
 __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(g3k_paged_args a) {
-    constexpr int ROWS = 64 * MT;
+    constexpr int ROWS = 16 * NW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int PER = ROWS / 4;     // workgroups per (block, head)
-    const int r4 = blockIdx.x % PER, x = blockIdx.x / PER;
+    const int row0 = blockIdx.x % (ROWS / MERGE_ROWS) * MERGE_ROWS, x = blockIdx.x / (ROWS / MERGE_ROWS);
     const int head = x % a.n_kv_heads, blk = x / a.n_kv_heads;
-    Unit u;
-    if (!find_block(a, blk, ROWS, lane, u)) return;
-    int kbeg, kend;
-    const int parts = split_keys(u, a.parts, 0, kbeg, kend);
-    const int row = r4 * 4 + wave;
-    if (parts == 1 || row >= u.count) return;
-    const long long slot = ((long long)blk * a.parts * a.n_kv_heads + head) * ROWS + row;
-    Joined j = {{0.f, 0.f, 0.f, 0.f}, M_NONE, 0.f};
-    join_parts(a.part_o + slot * D, a.part_ml + slot * 2, (long long)a.n_kv_heads * ROWS, parts, lane, j);
-    const int gs = __builtin_ctz(a.group);
-    float *out = a.out + ((long long)(u.run + (row >> gs)) * a.n_kv_heads * a.group + head * a.group + (row & (a.group - 1))) * D;
-    const float inv = j.l > 0.f || j.l != j.l ? 1.0f / j.l : 0.f;
-    *reinterpret_cast<f32x4 *>(out + 4 * lane) = j.o * inv;
+    const int T = ROWS / a.group, c = __builtin_amdgcn_readfirstlane(prompt_chunk(a, T, lane));
+    int blocks = 0, items = 0;     // before this run of sequences
+    for (int base = 0; base < a.s.num_seqs; base += 64) {
+        const Prompt mine = prompt_of(a, base + lane, T);
+        const int n = mine.blocks > 0 ? mine.items(a, c, T) : 0;
+        const int upto = wave_scan_int(mine.blocks, lane), iupto = wave_scan_int(n, lane);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(blk - blocks < upto);
+        if (!past) {
+            blocks += __builtin_amdgcn_readlane(upto, 63);
+            items += __builtin_amdgcn_readlane(iupto, 63);
+            continue;
+        }
+        const int at = __builtin_ctzll(past);
+        const Prompt p = uniform(mine, at);
+        const int rb = blk - blocks - (__builtin_amdgcn_readlane(upto, at) - p.blocks);
+        const int item0 = items + __builtin_amdgcn_readlane(iupto, at) - __builtin_amdgcn_readlane(n, at) + p.blocks - 1 - rb;
+        Unit u;
+        set_block(a, base + at, p, rb, T, u);
+        const int parts = block_chunks(u, c);
+        if (parts == 1) return;
+        const int gs = __builtin_ctz(a.group);
+        for (int row = row0 + wave; row < min(u.count, row0 + MERGE_ROWS); row += 4) {
+            Joined j;
+            j.clear();
+            int item = item0;
+            for (int q = 0; q < parts; q += 64) {
+                long long slot = 0;
+                const int k = min(parts - q, 64);
+                for (int i = 0; i < k; i++) {
+                    if (lane == i) slot = ((long long)min(item, a.items - 1) * a.n_kv_heads + head) * ROWS + row;
+                    item += p.blocks - p.first_with(q + i, c, T);
+                }
+                j.add(a, slot, k, lane);
+            }
+            j.store(a.out + ((long long)(u.run + (row >> gs)) * a.n_kv_heads * a.group + head * a.group + (row & (a.group - 1))) * D, lane);
+        }
+        return;
+    }
 }
 
 // ---- one query per sequence, shared prefixes ---------------------------------------
@@ -720,7 +881,6 @@ __device__ __forceinline__ int tail_begin(const g3k_paged_args &a, int len, int 
 // per sequence, the keys beyond.  Each is cut into chunks of `chunk` tiles so
 // that all of them make about a.budget items per KV head, whatever the
 // lengths: every wave adds the lengths up for itself.
-constexpr int MAX_TILES = G3K_PAGED_MAX_LEN / BK;
 template <int ROWS>
 __device__ int chunk_tiles(const g3k_paged_args &a, int lane) {
     float total = 0.f;      // rounded: 1e-4 is added below
@@ -789,7 +949,6 @@ __device__ Found find_chunk(const g3k_paged_args &a, int item, int per, int lane
             r.index = k % c;
             u.b = f;
             u.run = f + block * (ROWS / a.group);
-            u.first = 0;
             u.count = rows < ROWS ? rows : ROWS;
             u.pos = 0;
             u.kbeg = prefix_begin(a, p);
@@ -814,7 +973,6 @@ __device__ Found find_chunk(const g3k_paged_args &a, int item, int per, int lane
             r.chunks = __shfl(c, at);
             r.index = item - before - (__shfl(upto, at) - r.chunks);
             u.b = u.run = base + at;
-            u.first = 0;
             u.count = a.group;
             u.pos = 0;
             u.kbeg = __shfl(kb, at);
@@ -827,12 +985,14 @@ __device__ Found find_chunk(const g3k_paged_args &a, int item, int per, int lane
 }
 
 // Rows of a part: a prefix chunk's ROWS, a tail chunk's group heads.
-template <bool BF16, int MT>
-__global__ __launch_bounds__(256, 1) void paged_decode_kernel(g3k_paged_args a) {
+template <bool BF16, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void paged_decode_kernel(g3k_paged_args a) {
     __shared__ __align__(16) char lds[Lds<BF16>::BYTES];
-    __shared__ f32x4 factors[8];
-    constexpr int ROWS = 64 * MT;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ f32x2 factors[16];
+    __shared__ int exps[16];
+    constexpr int ROWS = 16 * NW;
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.n_kv_heads, item = blockIdx.x / a.n_kv_heads;
     const int per = __builtin_amdgcn_readfirstlane(chunk_tiles<ROWS>(a, lane));
     Unit u;
@@ -853,25 +1013,24 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(g3k_paged_args a) 
         dir[2 * u.run] = item;
         dir[2 * u.run + 1] = f.chunks;
     }
-    Rows<MT> s;
+    Rows s;
     const int gs = __builtin_ctz(a.group);
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int row = (wave * MT + mt) * 16 + (lane & 15);
+    {
+        const int row = wave * 16 + (lane & 15);
         const bool live = row < u.count;
         const int seq = u.run + (row >> gs), h = head * a.group + (row & (a.group - 1));
         const int len = live ? seq_len(a.s, seq) : 0;
-        s.hi[mt] = live ? min(len, u.kend) : INT_MAX;
-        s.lo[mt] = live ? max(len - a.window, u.kbeg) : 0;
-        load_query<MT>(a.q + ((long long)seq * a.n_kv_heads * a.group + h) * D, live, a.qscale, mt, lane, s);
+        s.hi = live ? min(len, u.kend) : INT_MAX;
+        s.lo = live ? max(len - a.window, u.kbeg) : 0;
+        load_query(a.q + ((long long)seq * a.n_kv_heads * a.group + h) * D, live, a.qscale, lane, s);
     }
-    begin_rows<MT>(s);
-    walk<BF16, MT>(a, head, u, lds, factors, wave, lane, s);
+    begin_rows(s);
+    walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, s);
+    G3K_RECOMPUTE(lane);      // no output address is kept through the walk
     int first;
     const bool whole = !f.prefix && f.chunks == 1 && seq_prefix(a, u.b, first) == 0;
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int row = (wave * MT + mt) * 16 + (lane & 15);
+    {
+        const int row = wave * 16 + (lane & 15);
         float *out = nullptr, *ml = nullptr;
         if (row < u.count) {
             if (whole) {
@@ -883,14 +1042,14 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(g3k_paged_args a) 
                 ml = a.part_ml + slot * 2;
             }
         }
-        store_row<MT>(s, mt, out, ml, lane);
+        store_row(s, out, ml, lane);
     }
 }
 
 // One wave per sequence and query head.
-template <int MT>
+template <int NW>
 __global__ __launch_bounds__(256) void paged_decode_merge_kernel(g3k_paged_args a) {
-    constexpr int ROWS = 64 * MT;
+    constexpr int ROWS = 16 * NW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = a.n_kv_heads * a.group;
     const long long id = (long long)blockIdx.x * 4 + wave;
@@ -906,47 +1065,55 @@ __global__ __launch_bounds__(256) void paged_decode_merge_kernel(g3k_paged_args 
     const int chunks = tail ? clampi(a.dir_tail[2 * b + 1], 0, a.items - at) : 0;
     if (p == 0 && chunks == 1) return;        // written by its one chunk
     const long long stride = (long long)a.n_kv_heads * a.part_rows;
-    Joined j = {{0.f, 0.f, 0.f, 0.f}, M_NONE, 0.f};
-    if (tail) {
-        const long long slot = ((long long)at * a.n_kv_heads + kvh) * a.part_rows + hg;
-        join_parts(a.part_o + slot * D, a.part_ml + slot * 2, stride, chunks, lane, j);
-    }
+    Joined j;
+    j.clear();
+    const auto add = [&](long long slot, int n) {
+        for (int q = 0; q < n; q += 64) j.add(a, slot + (q + min(lane, n - 1 - q)) * stride, min(n - q, 64), lane);
+    };
+    if (tail) add(((long long)at * a.n_kv_heads + kvh) * a.part_rows + hg, chunks);
     if (p > 0) {
         const int row = (b - first) * a.group + hg, lead = first + row / ROWS * (ROWS / a.group);
         const int item = clampi(a.dir_prefix[2 * lead], 0, a.items - 1);
-        const long long slot = ((long long)item * a.n_kv_heads + kvh) * a.part_rows + row % ROWS;
-        join_parts(a.part_o + slot * D, a.part_ml + slot * 2, stride, clampi(a.dir_prefix[2 * lead + 1], 0, a.items - item), lane, j);
+        add(((long long)item * a.n_kv_heads + kvh) * a.part_rows + row % ROWS, clampi(a.dir_prefix[2 * lead + 1], 0, a.items - item));
     }
-    const float inv = j.l > 0.f || j.l != j.l ? 1.0f / j.l : 0.f;
-    *reinterpret_cast<f32x4 *>(a.out + id * D + 4 * lane) = j.o * inv;
+    j.store(a.out + id * D, lane);
+}
+
+}  // namespace
+
+namespace {
+
+template <bool BF16, int NW>
+void launch_prefill(const g3k_paged_args &a, unsigned wgs, hipStream_t st) {
+    hipLaunchKernelGGL((paged_prefill_kernel<BF16, NW>), dim3(wgs), dim3(64 * NW), 0, st, a);
+    const unsigned merges = (unsigned)a.blocks * a.n_kv_heads * (16 * NW / MERGE_ROWS);
+    if (a.budget > 0) hipLaunchKernelGGL(paged_prefill_merge_kernel<NW>, dim3(merges), dim3(256), 0, st, a);
+}
+
+template <bool BF16, int NW>
+void launch_decode(const g3k_paged_args &a, unsigned wgs, hipStream_t st) {
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, NW>), dim3(wgs), dim3(64 * NW), 0, st, a);
+    const unsigned merges = ((unsigned)a.s.num_seqs * a.n_kv_heads * a.group + 3) / 4;
+    hipLaunchKernelGGL(paged_decode_merge_kernel<NW>, dim3(merges), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
 extern "C" int g3k_paged_prefill(const g3k_paged_args *a, void *stream) {
     hipStream_t st = (hipStream_t)stream;
-    const long long wgs = (long long)a->items * a->parts * a->n_kv_heads;
-    const long long merges = (long long)a->items * a->n_kv_heads * 16 * a->blocks;
-    if (wgs > INT_MAX || merges > INT_MAX) return (int)hipErrorInvalidValue;
-    const dim3 grid((unsigned)wgs), merge((unsigned)merges);
-    {
-        if (a->bf16) hipLaunchKernelGGL((paged_prefill_kernel<true, 1>), grid, dim3(256), 0, st, *a);
-        else hipLaunchKernelGGL((paged_prefill_kernel<false, 1>), grid, dim3(256), 0, st, *a);
-        if (a->parts > 1) hipLaunchKernelGGL(paged_prefill_merge_kernel<1>, merge, dim3(256), 0, st, *a);
-    }
+    const long long wgs = (long long)a->items * a->n_kv_heads;
+    if (wgs * 16 > INT_MAX) return (int)hipErrorInvalidValue;
+    const unsigned n = (unsigned)wgs;
+    if (a->waves == 8) a->bf16 ? launch_prefill<true, 8>(*a, n, st) : launch_prefill<false, 8>(*a, n, st);
+    else a->bf16 ? launch_prefill<true, 4>(*a, n, st) : launch_prefill<false, 4>(*a, n, st);
     return (int)hipGetLastError();
 }
 
 extern "C" int g3k_paged_decode(const g3k_paged_args *a, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     const long long wgs = (long long)a->items * a->n_kv_heads;
-    const long long merges = ((long long)a->s.num_seqs * a->n_kv_heads * a->group + 3) / 4;
-    if (wgs > INT_MAX || merges > INT_MAX) return (int)hipErrorInvalidValue;
-    const dim3 grid((unsigned)wgs), merge((unsigned)merges);
-    {
-        if (a->bf16) hipLaunchKernelGGL((paged_decode_kernel<true, 1>), grid, dim3(256), 0, st, *a);
-        else hipLaunchKernelGGL((paged_decode_kernel<false, 1>), grid, dim3(256), 0, st, *a);
-        hipLaunchKernelGGL(paged_decode_merge_kernel<1>, merge, dim3(256), 0, st, *a);
-    }
+    if (wgs > INT_MAX || (long long)a->s.num_seqs * a->n_kv_heads * a->group > INT_MAX) return (int)hipErrorInvalidValue;
+    if (a->waves == 8) a->bf16 ? launch_decode<true, 8>(*a, (unsigned)wgs, st) : launch_decode<false, 8>(*a, (unsigned)wgs, st);
+    else a->bf16 ? launch_decode<true, 4>(*a, (unsigned)wgs, st) : launch_decode<false, 4>(*a, (unsigned)wgs, st);
     return (int)hipGetLastError();
 }

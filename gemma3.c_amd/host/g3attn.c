@@ -2490,15 +2490,18 @@ int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pa
     g3k_paged_args a;
     fill_paged(c, layer, pages, batch, q, out, &a);
     const int Hkv = c->cfg.num_kv_heads;
-    a.blocks = 1;
-    const int rows = 64 * a.blocks;
-    a.items = prefill_blocks(batch, c->group, rows);
-    /* few blocks: their keys are split until about two workgroups a CU are there */
-    long long parts = 2LL * c->n_cu / ((long long)a.items * Hkv);
-    a.parts = parts < 1 ? 1 : parts > 16 ? 16 : (int)parts;
+    a.waves = 8;
+    if ((long long)prefill_blocks(batch, c->group, 128) * Hkv < c->n_cu) a.waves = 4;
+    const int rows = 16 * a.waves;
+    a.blocks = a.items = prefill_blocks(batch, c->group, rows);
     hipSetDevice(c->device);
-    if (a.parts > 1) {
-        const size_t n = (size_t)a.items * a.parts * Hkv * rows, ob = align256(n * D * sizeof(float));
+    /* Where blocks are many their different lengths even out over the CUs;
+     * else the long ones' keys are cut. */
+    if ((long long)a.blocks * Hkv <= 8LL * c->n_cu) {
+        a.budget = (3 * c->n_cu / 2 + Hkv - 1) / Hkv;
+        a.min_tiles = 8;
+        a.items = a.blocks + a.budget + 1;
+        const size_t n = (size_t)a.items * Hkv * rows, ob = align256(n * D * sizeof(float));
         unsigned char *ws;
         PAGED_TRY(paged_scratch(c, ob + n * 2 * sizeof(float), fn, &ws));
         a.part_o = (float *)ws;
@@ -2526,8 +2529,8 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
         a.group_start = prefixes->group_start;
         a.prefix_len = prefixes->prefix_len;
     }
-    a.blocks = 1;
-    const int rows = 64 * a.blocks;
+    a.waves = a.n_groups && B * c->group > 64 * a.n_groups ? 8 : 4;
+    const int rows = 16 * a.waves;
     /* items per KV head: one workgroup a CU, and one more for every run of
      * keys (its last chunk is a part one) */
     const int units = B + (a.n_groups ? a.n_groups + B * c->group / rows : 0);

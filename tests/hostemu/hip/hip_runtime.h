@@ -99,6 +99,7 @@ hipError_t hipOccupancyMaxActiveBlocksPerMultiprocessor(int *n, K, int, size_t) 
 // The library's explicit waits for buffer -> LDS fetches (see the top).
 #define G3K_WAIT_VMEM() hostemu::complete_fetches(0)
 #define G3K_WAIT_BARRIER(n) (hostemu::complete_fetches(n), hostemu::machine()->block.wait())
+#define G3K_RECOMPUTE(x) ((void)(x))
 #define G3K_ORDER_FENCE() ((void)hostemu::machine()->current->fence++)
 // The emulated machine deals workgroup i to XCD i mod 8, as the MI355X
 // dispatcher does.
@@ -455,6 +456,13 @@ inline int hostemu_readfirstlane(int v) {
     return (int)r;
 }
 #define __builtin_amdgcn_readfirstlane hostemu_readfirstlane
+
+inline int hostemu_readlane(int v, int lane) {
+    uint32_t r, unused;
+    hostemu::exchange((uint32_t)v, 0, lane, &r, &unused);
+    return (int)r;
+}
+#define __builtin_amdgcn_readlane hostemu_readlane
 
 inline uint64_t hostemu_ballot_w64(bool p) {
     hostemu::Wave &w = hostemu::machine()->waves[hostemu::t_wave];
