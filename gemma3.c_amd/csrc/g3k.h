@@ -390,20 +390,23 @@ typedef struct {
 } g3k_paged_write_args;
 int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
 
+#define G3K_PAGED_DECODE_ROWS 128   /* of a group, per workgroup on its prefix */
+
 /* Attention of packed tokens (prefill) or of one token per sequence (decode)
- * over pages; q and out [total_q][heads][D].  waves: per workgroup, 4 or 8, 16
- * rows each.
- * Prefill: blocks bounds the row blocks of the batch, sum over sequences of
+ * over pages; q and out [total_q][heads][D].
+ * Prefill: waves per workgroup, 4 or 8, 16 rows each; blocks bounds the row blocks of the batch, sum over sequences of
  * ceil(tokens * group / (16 waves)).  The keys of the longest are cut into
  * chunks of at least min_tiles 32-key tiles, to about `budget` items per KV
  * head and at most `items` (blocks + budget + 1); the parts [items][n_kv_heads]
  * [16 waves] rows are joined by a second launch.  budget 0: not cut, items =
  * blocks.
  * Decode: group i's members [group_start[i], group_start[i + 1]) share their
- * first prefix_len[i] positions, read once through the first member's table.
+ * first prefix_len[i] positions, read once per G3K_PAGED_DECODE_ROWS rows
+ * through the first member's table.
  * The keys are cut into about `budget` chunks per KV head, at most `items`,
- * of at least min_tiles 32-key tiles; parts [items][n_kv_heads][part_rows]
- * rows, found through the directories dir_prefix and dir_tail [num_seqs][2]. */
+ * of at least min_tiles 32-key tiles; with `pack`, short sequences are one
+ * wave's work.  Parts [items][n_kv_heads][part_rows]
+ * rows, found through the directories dir_prefix and dir_tail [num_seqs][4]. */
 typedef struct {
     g3k_paged_seqs s;
     const void *k, *v;
@@ -416,7 +419,7 @@ typedef struct {
     float *part_o, *part_ml;   /* D floats, and (max, sum), per row */
     int n_groups;
     const int *group_start, *prefix_len;
-    int budget, min_tiles, part_rows;
+    int budget, min_tiles, part_rows, pack;
     int *dir_prefix, *dir_tail;
 } g3k_paged_args;
 int g3k_paged_prefill(const g3k_paged_args *a, void *stream);

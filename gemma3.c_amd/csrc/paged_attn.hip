@@ -687,7 +687,7 @@ __device__ bool find_item(const g3k_paged_args &a, int item, int c, int T, int l
     for (int base = 0; base < a.s.num_seqs; base += 64) {
         const Prompt mine = prompt_of(a, base + lane, T);
         const int n = mine.blocks > 0 ? mine.items(a, c, T) : 0;
-        const int upto = wave_scan_int(n, lane);
+        const int upto = wave_scan_int(n);
         const uint64_t past = __builtin_amdgcn_ballot_w64(item - before < upto);
         if (past) {
             const int at = __builtin_ctzll(past);
@@ -764,25 +764,40 @@ struct Joined {
         m = M_NONE;
         l = 0.f;
     }
-    // Adds n <= 64 parts: lane i's slot is part i's row.  The statistics are
-    // one load a lane.
+    // Adds n <= 64 parts (n > 0): lane i's slot is part i's row.  The
+    // statistics are one load a lane; the first outputs are on their way with
+    // them.
     __device__ __forceinline__ void add(const g3k_paged_args &a, long long slot, int n, int lane) {
+        constexpr int AT = 8;
+        f32x4 x[AT];
+        const auto fetch = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < AT; i++) {
+                const int j = min(i0 + i, n - 1);
+                const long long sj = (long long)(unsigned)__builtin_amdgcn_readlane((int)slot, j) |
+                                     (long long)__builtin_amdgcn_readlane((int)(slot >> 32), j) << 32;
+                x[i] = *reinterpret_cast<const f32x4 *>(a.part_o + sj * D + 4 * lane);
+            }
+        };
         float pm = M_NONE, pl = 0.f;
         if (lane < n) {
-            pm = a.part_ml[2 * slot];
-            pl = a.part_ml[2 * slot + 1];
+            const f32x2 st = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * slot);
+            pm = st.x;
+            pl = st.y;
         }
+        fetch(0);
         const float top = fmaxf(wave_max(pm), m);
         const float w = pl * fast_exp2(pm - top), keep = fast_exp2(m - top);
         o *= keep;
         l = l * keep + wave_sum(w);
         m = top;
-#pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
-            const long long si = (long long)(unsigned)__builtin_amdgcn_readlane((int)slot, i) |
-                                 (long long)__builtin_amdgcn_readlane((int)(slot >> 32), i) << 32;
-            o += wi * *reinterpret_cast<const f32x4 *>(a.part_o + si * D + 4 * lane);
+        for (int i0 = 0;;) {
+#pragma unroll
+            for (int i = 0; i < AT; i++)
+                if (i0 + i < n) o += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(i0 + i, 63))) * x[i];
+            i0 += AT;
+            if (i0 >= n) break;
+            fetch(i0);
         }
     }
     __device__ __forceinline__ void store(float *out, int lane) const {
@@ -805,7 +820,7 @@ __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(g3k_paged_args
     for (int base = 0; base < a.s.num_seqs; base += 64) {
         const Prompt mine = prompt_of(a, base + lane, T);
         const int n = mine.blocks > 0 ? mine.items(a, c, T) : 0;
-        const int upto = wave_scan_int(mine.blocks, lane), iupto = wave_scan_int(n, lane);
+        const int upto = wave_scan_int(mine.blocks), iupto = wave_scan_int(n);
         const uint64_t past = __builtin_amdgcn_ballot_w64(blk - blocks < upto);
         if (!past) {
             blocks += __builtin_amdgcn_readlane(upto, 63);
@@ -877,116 +892,495 @@ __device__ __forceinline__ int tail_begin(const g3k_paged_args &a, int len, int 
     return lo > p ? lo : p;
 }
 
-// The work of a decode: per group and 64 MT members' rows, the prefix's keys;
-// per sequence, the keys beyond.  Each is cut into chunks of `chunk` tiles so
-// that all of them make about a.budget items per KV head, whatever the
-// lengths: every wave adds the lengths up for itself.
-template <int ROWS>
-__device__ int chunk_tiles(const g3k_paged_args &a, int lane) {
-    float total = 0.f;      // rounded: 1e-4 is added below
-    int units = 0;
-    for (int base = 0; base < a.n_groups; base += 64) {
-        float t = 0.f;
-        int n = 0;
-        if (base + lane < a.n_groups) {
-            int f, e;
-            const int p = group_prefix(a, base + lane, f, e);
-            if (p > 0) {
-                n = ((e - f) * a.group + ROWS - 1) / ROWS;
-                t = (float)n * (float)tiles_of(prefix_begin(a, p), p);
-            }
+// The work of a decode: per group and ROWS of its members' rows, the prefix's
+// keys; per sequence, the keys beyond.  A wave's lanes look at 64 groups or
+// sequences at a time; the first 64 of each stay in registers.
+struct GroupLane {
+    int first, end, p, blocks, tiles;
+};
+struct SeqLane {
+    int kbeg, len, tiles, shares;
+    int alone;       // short enough for one wave (tiles is 0 then)
+};
+
+__device__ __forceinline__ GroupLane group_lane(const g3k_paged_args &a, int i, int rows) {
+    GroupLane g = {0, 0, 0, 0, 0};
+    if (i < a.n_groups) {
+        g.p = group_prefix(a, i, g.first, g.end);
+        if (g.p > 0) {
+            g.blocks = ((g.end - g.first) * a.group + rows - 1) / rows;
+            g.tiles = tiles_of(prefix_begin(a, g.p), g.p);
         }
-        total += wave_sum(t);
-        units += wave_sum_int(n);
     }
-    for (int base = 0; base < a.s.num_seqs; base += 64) {
-        float t = 0.f;
-        if (base + lane < a.s.num_seqs) {
-            int f;
-            const int len = seq_len(a.s, base + lane), p = seq_prefix(a, base + lane, f);
-            t = (float)tiles_of(tail_begin(a, len, p), len);
+    return g;
+}
+// Where there are more sequences than CUs, one with at most this many tiles is
+// one wave's work, and a workgroup takes as many of them as it has waves.
+constexpr int ALONE_TILES = 4;
+__device__ __forceinline__ SeqLane seq_lane(const g3k_paged_args &a, int b) {
+    SeqLane s = {0, 0, 0, 0, 0};
+    if (b < a.s.num_seqs) {
+        int first;
+        s.len = seq_len(a.s, b);
+        s.shares = seq_prefix(a, b, first);
+        s.kbeg = tail_begin(a, s.len, s.shares);
+        s.tiles = tiles_of(s.kbeg, s.len);
+        if (a.pack && s.tiles > 0 && s.tiles <= ALONE_TILES) {
+            s.alone = s.tiles;
+            s.tiles = 0;
         }
-        total += wave_sum(t);
     }
-    units += a.s.num_seqs;
-    const int room = a.budget - units > 1 ? a.budget - units : 1;
-    const float c = total * 1.0001f / (float)room + 1.0f;
-    return c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
+    return s;
 }
 
-// Finds chunk `item`: its unit (keys and rows), whether it is a prefix's, and
-// how many chunks its unit has.  index: the chunk's number within the unit.
+// The units' keys are cut into chunks of about equal work, as many as make at
+// most a.budget items per KV head, whatever the lengths: every wave adds the
+// lengths up for itself, then finds its item.  One item more than there are
+// CUs costs a second round of workgroups (8 unrelated sequences, 313 tiles: 36
+// us with 67 items a head, 21 with 64), so where the lengths are all in
+// registers the chunks are lengthened until the count fits.
+struct DecodePlan {
+    GroupLane g0;
+    SeqLane s0;
+    int per;        // tiles a chunk, at most; a prefix's tile counts as two
+    int alone;      // sequences that are one wave's work
+    __device__ __forceinline__ static int chunks(int tiles, int per) { return (tiles + per - 1) / per; }
+    __device__ __forceinline__ int prefix_chunks(int tiles) const { return chunks(tiles, max((per + 1) >> 1, 1)); }
+
+    __device__ __forceinline__ void begin(const g3k_paged_args &a, int rows, int waves, int lane) {
+        g0 = group_lane(a, lane, rows);
+        s0 = seq_lane(a, lane);
+        const bool all = a.n_groups <= 64 && a.s.num_seqs <= 64;
+        float total = 2.f * (float)g0.blocks * (float)g0.tiles + (float)s0.tiles;   // rounded: 1e-4 is added below
+        int units = g0.blocks;
+        alone = s0.alone > 0;
+        for (int base = 64; base < a.n_groups; base += 64) {
+            const GroupLane g = group_lane(a, base + lane, rows);
+            total += 2.f * (float)g.blocks * (float)g.tiles;
+            units += g.blocks;
+        }
+        for (int base = 64; base < a.s.num_seqs; base += 64) {
+            const SeqLane q = seq_lane(a, base + lane);
+            total += (float)q.tiles;
+            alone += q.alone > 0;
+        }
+        total = wave_sum(total);
+        alone = a.pack ? wave_sum_int(alone) : 0;
+        const int packs = (alone + waves - 1) / waves;
+        units = a.s.num_seqs - alone + (a.n_groups ? wave_sum_int(units) : 0);
+        const int budget = max(a.budget - packs, 1);
+        const int room = all ? budget : max(budget - units, budget / 2);
+        const float c = total * 1.0001f / (float)max(room, 1) + 1.0f;
+        per = c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
+        if (!all) return;
+        for (int i = 0; i < 16; i++) {
+            if (wave_sum_int(g0.blocks * prefix_chunks(g0.tiles) + chunks(s0.tiles, per)) <= budget) break;
+            per += max(per >> 3, 1);
+        }
+    }
+};
+
+// Chunk `item`: its unit, keys and rows, whether it is a prefix's, how many
+// chunks its unit has, which of them it is, and whether its sequence shares.
+// Or a pack: `alone`, and each wave finds its own sequence (chunks 0: none).
 struct Found {
-    bool any, prefix;
+    bool any, prefix, alone, shares;
     int chunks, index;
 };
-template <int ROWS>
-__device__ Found find_chunk(const g3k_paged_args &a, int item, int per, int lane, Unit &u) {
-    Found r = {false, false, 0, 0};
+__device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int item, int rows, int wave, int waves, int lane, Unit &u) {
+    Found r = {false, false, false, false, 0, 0};
+    const auto at = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+    // the chunk's keys: its even share of the unit's tiles
+    const auto keys = [&](int kbeg, int kend, int tiles) {
+        const int each = (tiles + r.chunks - 1) / r.chunks, t0 = kbeg / BK + r.index * each;
+        u.kbeg = max(kbeg, t0 * BK);
+        u.kend = min(kend, (t0 + each) * BK);
+    };
     int before = 0;
     for (int base = 0; base < a.n_groups; base += 64) {
-        int f = 0, e = 0, p = 0, n = 0, c = 0;
-        if (base + lane < a.n_groups) {
-            p = group_prefix(a, base + lane, f, e);
-            if (p > 0) {
-                c = (tiles_of(prefix_begin(a, p), p) + per - 1) / per;
-                n = ((e - f) * a.group + ROWS - 1) / ROWS;
-            }
-        }
-        const int upto = wave_scan_int(n * c, lane);
+        const GroupLane g = base ? group_lane(a, base + lane, rows) : plan.g0;
+        const int c = plan.prefix_chunks(g.tiles);
+        const int upto = wave_scan_int(g.blocks * c);
         const uint64_t past = __builtin_amdgcn_ballot_w64(item - before < upto);
         if (past) {
-            const int at = __builtin_ctzll(past);
-            c = __shfl(c, at);
-            n = __shfl(n, at);
-            f = __shfl(f, at);
-            e = __shfl(e, at);
-            p = __shfl(p, at);
-            const int k = item - before - (__shfl(upto, at) - n * c);
-            const int block = k / c, rows = (e - f) * a.group - block * ROWS;
+            const int l = __builtin_ctzll(past);
+            const int first = at(g.first, l), end = at(g.end, l), p = at(g.p, l);
+            r.chunks = at(c, l);
+            const int k = item - before - (at(upto, l) - at(g.blocks, l) * r.chunks);
+            const int block = k / r.chunks, left = (end - first) * a.group - block * rows;
             r.any = r.prefix = true;
-            r.chunks = c;
-            r.index = k % c;
-            u.b = f;
-            u.run = f + block * (ROWS / a.group);
-            u.count = rows < ROWS ? rows : ROWS;
+            r.index = k % r.chunks;
+            u.b = first;
+            u.run = first + block * (rows / a.group);
+            u.count = left < rows ? left : rows;
             u.pos = 0;
-            u.kbeg = prefix_begin(a, p);
-            u.kend = p;
+            keys(prefix_begin(a, p), p, at(g.tiles, l));
             return r;
         }
-        before += __shfl(upto, 63);
+        before += at(upto, 63);
     }
     for (int base = 0; base < a.s.num_seqs; base += 64) {
-        int kb = 0, len = 0, c = 0;
-        if (base + lane < a.s.num_seqs) {
-            int f;
-            len = seq_len(a.s, base + lane);
-            kb = tail_begin(a, len, seq_prefix(a, base + lane, f));
-            c = (tiles_of(kb, len) + per - 1) / per;
-        }
-        const int upto = wave_scan_int(c, lane);
+        const SeqLane s = base ? seq_lane(a, base + lane) : plan.s0;
+        const int c = DecodePlan::chunks(s.tiles, plan.per);
+        const int upto = wave_scan_int(c);
         const uint64_t past = __builtin_amdgcn_ballot_w64(item - before < upto);
         if (past) {
-            const int at = __builtin_ctzll(past);
+            const int l = __builtin_ctzll(past);
             r.any = true;
-            r.chunks = __shfl(c, at);
-            r.index = item - before - (__shfl(upto, at) - r.chunks);
-            u.b = u.run = base + at;
+            r.chunks = at(c, l);
+            r.index = item - before - (at(upto, l) - r.chunks);
+            r.shares = at(s.shares, l) > 0;
+            u.b = u.run = base + l;
             u.count = a.group;
             u.pos = 0;
-            u.kbeg = __shfl(kb, at);
-            u.kend = __shfl(len, at);
+            keys(at(s.kbeg, l), at(s.len, l), at(s.tiles, l));
             return r;
         }
-        before += __shfl(upto, 63);
+        before += at(upto, 63);
+    }
+    if ((item - before) * waves >= plan.alone) return r;
+    r.any = r.alone = true;
+    const int k = (item - before) * waves + wave;
+    u.b = u.run = u.pos = u.kbeg = u.kend = 0;
+    u.count = a.group;
+    before = 0;
+    for (int base = 0; base < a.s.num_seqs; base += 64) {
+        const SeqLane s = base ? seq_lane(a, base + lane) : plan.s0;
+        const int upto = wave_scan_int(s.alone > 0);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(k - before < upto);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            r.chunks = 1;
+            r.shares = at(s.shares, l) > 0;
+            u.b = u.run = base + l;
+            u.kbeg = at(s.kbeg, l);
+            u.kend = at(s.len, l);
+            return r;
+        }
+        before += at(upto, 63);
     }
     return r;
 }
 
-// Rows of a part: a prefix chunk's ROWS, a tail chunk's group heads.
+// A tail chunk: one sequence's keys, for the (at most four) query heads of the
+// KV head.  There is nothing to share between waves, so each takes 16 keys of
+// its own at a time, straight from memory to registers to the matrix units: a
+// K lane holds one key's share of every dim step's operand, a V lane four dims
+// (bf16: eight) of its lane group's four keys, which are operand lanes of as
+// many dim blocks, and S^T's registers are P's operand.  While the scores of
+// a step are taken its V is on its way, while its values are the next K: 32
+// KiB in flight a wave (bf16: 16).  The waves of a workgroup take the steps of
+// one chunk in turn, or each all steps of a short sequence of its own.  The
+// queries' four rows lie in LDS as operand lanes, which the other 12 columns
+// of the operand read too: those columns of S^T and O^T are never used.
+template <bool BF16>
+struct Step {
+    static constexpr int ROW = D * (BF16 ? 2 : 4);
+    static constexpr int N = BF16 ? 8 : 16;        // 16-byte loads a lane and matrix
+    u32x4 k[N], v[N];
+    // Lane (c, g)'s offsets from the step's first row; rows outside [0, rows)
+    // of it are the nearest one's.
+    __device__ __forceinline__ void load_k(const char *base, int rs, int first, int end, int lane) {
+        const char *row = base + clampi(lane & 15, first, end - 1) * rs + (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < N; i++) k[i] = *reinterpret_cast<const u32x4 *>(row + i * 64);
+    }
+    __device__ __forceinline__ void load_v(const char *base, int rs, int first, int end, int lane) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const char *row = base + clampi(4 * (lane >> 4) + i, first, end - 1) * rs + (lane & 15) * 16;
+#pragma unroll
+            for (int T = 0; T < N / 4; T++) v[T * 4 + i] = *reinterpret_cast<const u32x4 *>(row + T * 256);
+        }
+    }
+};
+
+__device__ __forceinline__ float bf16_of(const u32x4 &x, int i) {
+    const unsigned u = x[i >> 1];
+    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+}
+__device__ __forceinline__ float f32_of(const u32x4 &x, int i) { return __uint_as_float(x[i]); }
+
+template <bool BF16>
+__device__ __forceinline__ float step_max(const u32x4 (&x)[BF16 ? 8 : 16]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 8 : 16); i++)
+#pragma unroll
+        for (int e = 0; e < (BF16 ? 8 : 4); e += 2)
+            m = BF16 ? fmaxf(fmaxf(m, fabsf(bf16_of(x[i], e))), fabsf(bf16_of(x[i], e + 1)))
+                     : fmaxf(fmaxf(m, fabsf(f32_of(x[i], e))), fabsf(f32_of(x[i], e + 1)));
+    return wave_max(m);
+}
+
+// The dim of element i of dim step kk's operand lane of group g: K's loads are
+// 64 bytes of a row a group of lanes.
+template <bool BF16>
+__device__ __forceinline__ int step_dim(int kk, int g, int i) {
+    return BF16 ? 32 * kk + 8 * g + i : 32 * kk + 16 * (i >> 2) + 4 * g + (i & 3);
+}
+
+// O^T of one row, as the waves of a workgroup leave it.
+struct Tail {
+    f32x4 o[16];
+    float m, l;
+    int ev;
+};
+
+// This wave takes steps step0, step0 + stride, ...; queries: 4 KiB, of which it
+// stores the dim steps kk with kk % stride == step0.
+template <bool BF16>
+__device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, const Unit &u, char *queries, int step0, int stride,
+                                          int lane, Tail &s) {
+    constexpr int ROW = Step<BF16>::ROW;
+    const int g = lane >> 4, c = lane & 15;
+    s.m = M_NONE;
+    s.l = 0.f;
+    s.ev = E_NONE;
+#pragma unroll
+    for (int d = 0; d < 16; d++) s.o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int j0 = u.kbeg & ~15, steps = (u.kend - j0 + 15) / 16;
+    const int *table = a.s.page_table + (long long)u.b * a.s.table_stride;
+    const int shift = a.s.page_shift, mask = (1 << shift) - 1, last = max(u.kend - 1, 0) >> shift;
+    const long long head_off = ((long long)head << shift) * D;
+    const char *kb = static_cast<const char *>(a.k) + head_off * (ROW / D), *vb = static_cast<const char *>(a.v) + head_off * (ROW / D);
+    // lane i: the page of this wave's step base + i
+    const auto look = [&](int base) { return table[min((j0 + 16 * (step0 + stride * (base + lane))) >> shift, last)]; };
+    int ids = look(0);
+    // the queries, row c of the group's heads: asked for before K and V, which
+    // would otherwise have to arrive first
+    const float *q = a.q + (((long long)u.run * a.n_kv_heads + head) * a.group + c) * D;
+    const bool live = c < a.group;
+    f32x4 xq[8][2];
+#pragma unroll
+    for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            xq[kk][i >> 2] = live ? *reinterpret_cast<const f32x4 *>(q + step_dim<BF16>(kk, g, i)) : z;
+        }
+    // a step's first row from the head's first page, or rows of zeros
+    struct Where {
+        long long off;
+        int rs;
+    };
+    const auto where = [&](int n) {
+        if ((n & 63) == 0 && n) ids = look(n);
+        const unsigned page = __builtin_amdgcn_readlane(ids, n & 63);
+        const int j = j0 + 16 * (step0 + stride * n);
+        Where w;
+        w.off = (long long)(((unsigned long long)page * (unsigned)a.page_stride + (unsigned)((j & mask) * D)) * (ROW / D));
+        w.rs = page < (unsigned)a.num_pages ? ROW : 0;
+        return w;
+    };
+    Step<BF16> x;
+    const int mine = steps > step0 ? (steps - step0 + stride - 1) / stride : 0;
+    const auto begin = [&](int n) { return max(u.kbeg - (j0 + 16 * (step0 + stride * n)), 0); };
+    const auto end = [&](int n) { return min(u.kend - (j0 + 16 * (step0 + stride * n)), 16); };
+    const char *zeros = reinterpret_cast<const char *>(zero_row);
+    Where w = {0, 0};
+    if (mine > 0) {
+        w = where(0);
+        x.load_k(w.rs ? kb + w.off : zeros, w.rs, begin(0), end(0), lane);
+        x.load_v(w.rs ? vb + w.off : zeros, w.rs, begin(0), end(0), lane);
+    }
+    float qfac;
+    {
+        float m = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(xq[kk][i >> 2][i & 3]));
+        const int e = block_exponent(col4_max(m));
+        const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
+        qfac = __builtin_amdgcn_ldexpf(a.qscale, e - X_EXP);
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+            if (kk % stride != step0 || c >= 4) continue;
+            half8 h, l;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v hh, ll;
+                split2(xq[kk][i >> 2][i & 3], xq[kk][i >> 2][(i & 3) + 1], sc, hh, ll);
+                h[i] = hh.x;
+                h[i + 1] = hh.y;
+                l[i] = ll.x;
+                l[i + 1] = ll.y;
+            }
+            *reinterpret_cast<half8 *>(queries + kk * 512 + (4 * g + c) * 16) = h;
+            *reinterpret_cast<half8 *>(queries + kk * 512 + 256 + (4 * g + c) * 16) = l;
+        }
+    }
+    G3K_WAIT_BARRIER(63);
+    for (int n = 0; n < mine; n++) {
+        const int first = begin(n), fin = end(n);
+        const bool gone = w.rs == 0;
+        G3K_RECOMPUTE(lane);
+        const int ek = block_exponent(step_max<BF16>(x.k));
+        const float sk = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ek);
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f}, sx = sc, sy = sc;
+        const char *qp = queries + (4 * (lane >> 4) + (lane & 3)) * 16;
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+            const half8 qh = *reinterpret_cast<const half8 *>(qp + kk * 512);
+            const half8 ql = *reinterpret_cast<const half8 *>(qp + kk * 512 + 256);
+            half8 h, l;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v hh, ll;
+                if constexpr (BF16) {
+                    hh = cvt2(bf16_of(x.k[kk], i) * sk, bf16_of(x.k[kk], i + 1) * sk);
+                } else {
+                    split2(f32_of(x.k[2 * kk + (i >> 2)], i & 3), f32_of(x.k[2 * kk + (i >> 2)], (i & 3) + 1), sk, hh, ll);
+                    l[i] = ll.x;
+                    l[i + 1] = ll.y;
+                }
+                h[i] = hh.x;
+                h[i + 1] = hh.y;
+            }
+            sc = mfma(h, qh, sc);
+            sx = mfma(h, ql, sx);
+            if constexpr (!BF16) sy = mfma(l, qh, sy);
+            KEEP_OPERANDS();
+        }
+        if (n + 1 < mine) {
+            w = where(n + 1);
+            x.load_k(w.rs ? kb + w.off : zeros, w.rs, begin(n + 1), end(n + 1), lane);
+        }
+        sc += sx;
+        if constexpr (!BF16) sc += sy;
+        const float f = qfac * __builtin_amdgcn_ldexpf(1.0f, ek - X_EXP);
+        float t = M_NONE;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int j = 4 * g + r;
+            sc[r] = gone || j < first || j >= fin ? -INFINITY : sc[r] * f;
+            t = fmaxf(t, sc[r]);
+        }
+        t = col4_max(t);
+        const int ev = block_exponent(step_max<BF16>(x.v));
+        const bool up = t > s.m + LAZY;
+        if (__builtin_amdgcn_ballot_w64(up) || ev > s.ev) {
+            const float m = up ? t : s.m;
+            float keep = fast_exp2(s.m - m);
+            s.m = m;
+            s.l *= keep;
+            if (ev > s.ev) {
+                keep *= s.ev == E_NONE ? 0.f : __builtin_amdgcn_ldexpf(1.0f, s.ev - ev - 2);
+                s.ev = ev + 2;
+            }
+#pragma unroll
+            for (int d = 0; d < 16; d++) s.o[d] *= keep;
+        }
+        const float pf = __builtin_amdgcn_ldexpf(1.0f, P_EXP + ev - s.ev), sv = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ev);
+        half4v ph, pl;
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            const float p0 = fast_exp2(sc[r] - s.m), p1 = fast_exp2(sc[r + 1] - s.m);
+            s.l += p0 + p1;
+            half2v h, l;
+            split2(p0, p1, pf, h, l);
+            ph[r] = h.x;
+            ph[r + 1] = h.y;
+            pl[r] = l.x;
+            pl[r + 1] = l.y;
+        }
+        constexpr int PER = BF16 ? 8 : 4;       // dims a lane and load
+        half4v lo = {};
+#pragma unroll
+        for (int d = 0; d < 16; d++) {
+            const int T = d / PER, e = d % PER;
+            half4v h, l;
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                half2v hh, ll;
+                if constexpr (BF16) {
+                    hh = cvt2(bf16_of(x.v[T * 4 + i], e) * sv, bf16_of(x.v[T * 4 + i + 1], e) * sv);
+                } else {
+                    split2(f32_of(x.v[T * 4 + i], e), f32_of(x.v[T * 4 + i + 1], e), sv, hh, ll);
+                    l[i] = ll.x;
+                    l[i + 1] = ll.y;
+                }
+                h[i] = hh.x;
+                h[i + 1] = hh.y;
+            }
+            s.o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(h, ph, s.o[d], 0, 0, 0);
+            if constexpr (!BF16) {
+                if (d > 0) s.o[d - 1] = __builtin_amdgcn_mfma_f32_16x16x16f16(lo, ph, s.o[d - 1], 0, 0, 0);
+                lo = l;
+            }
+            s.o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(h, pl, s.o[d], 0, 0, 0);
+        }
+        if constexpr (!BF16) s.o[15] = __builtin_amdgcn_mfma_f32_16x16x16f16(lo, ph, s.o[15], 0, 0, 0);
+        if (n + 1 < mine) x.load_v(w.rs ? vb + w.off : zeros, w.rs, begin(n + 1), end(n + 1), lane);
+    }
+}
+
+// Stores a tail's row of this lane (c < group): rows stride D apart, normalised.
+template <bool BF16>
+__device__ __forceinline__ void store_tail_rows(const Tail &s, float inv, float *rows, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const int e = s.ev == E_NONE ? 0 : s.ev - X_EXP - P_EXP;
+    constexpr int PER = BF16 ? 8 : 4;
+#pragma unroll
+    for (int T = 0; T < 16 / PER; T++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < PER; t += 4) {
+                f32x4 x;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = __builtin_amdgcn_ldexpf(s.o[PER * T + t + i][r] * inv, e);
+                *reinterpret_cast<f32x4 *>(rows + c * D + 16 * PER * T + PER * (4 * g + r) + t) = x;
+            }
+}
+
+// Joins the waves' shares of a tail and stores the group's rows: to out, or a
+// part with its (max, sum).
 template <bool BF16, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void paged_decode_kernel(g3k_paged_args a) {
+__device__ __forceinline__ void store_tail(const g3k_paged_args &a, Tail &s, char *lds, int wave, int lane, float *out, float *ml) {
+    float *ws = reinterpret_cast<float *>(lds);            // [wave][row][D], then [wave][row] of (max, sum)
+    float *st = ws + NW * 4 * D;
+    const int c = lane & 15, g = lane >> 4;
+    const float l = col4_sum(s.l);
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    __syncthreads();           // the queries in LDS have been read
+    if (c < a.group) {
+        store_tail_rows<BF16>(s, inv, ws + wave * 4 * D, lane);
+        if (g == 0) {
+            st[2 * (wave * 4 + c)] = s.m;
+            st[2 * (wave * 4 + c) + 1] = l;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.group * (D / 4); i += 64 * NW) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        float top = M_NONE;
+#pragma unroll
+        for (int w = 0; w < NW; w++) top = fmaxf(top, st[2 * (w * 4 + row)]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float k = st[2 * (w * 4 + row) + 1] * fast_exp2(st[2 * (w * 4 + row)] - top);
+            sum += k;
+            o += k * *reinterpret_cast<const f32x4 *>(ws + (w * 4 + row) * D + d);
+        }
+        const float y = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+        *reinterpret_cast<f32x4 *>(out + row * D + d) = o * y;
+        if (ml && d == 0) {
+            ml[2 * row] = top;
+            ml[2 * row + 1] = sum;
+        }
+    }
+}
+
+// Rows of a part: a prefix chunk's ROWS, a tail chunk's group heads.
+constexpr int DECODE_WAVES = G3K_PAGED_DECODE_ROWS / 16;
+template <bool BF16>
+__global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_decode_kernel(g3k_paged_args a) {
+    constexpr int NW = DECODE_WAVES;
     __shared__ __align__(16) char lds[Lds<BF16>::BYTES];
     __shared__ f32x2 factors[16];
     __shared__ int exps[16];
@@ -994,24 +1388,40 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_decode_kernel(g3k_paged
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.n_kv_heads, item = blockIdx.x / a.n_kv_heads;
-    const int per = __builtin_amdgcn_readfirstlane(chunk_tiles<ROWS>(a, lane));
+    DecodePlan plan;
+    plan.begin(a, ROWS, NW, lane);
     Unit u;
-    Found f = find_chunk<ROWS>(a, item, per, lane, u);
+    const Found f = find_chunk(a, plan, item, ROWS, wave, NW, lane, u);
     if (!f.any) return;
-    u.b = __builtin_amdgcn_readfirstlane(u.b);
-    u.run = __builtin_amdgcn_readfirstlane(u.run);
-    u.count = __builtin_amdgcn_readfirstlane(u.count);
-    f.chunks = __builtin_amdgcn_readfirstlane(f.chunks);
-    f.index = __builtin_amdgcn_readfirstlane(f.index);
-    const int t0 = __builtin_amdgcn_readfirstlane(u.kbeg) / BK, kb = (t0 + f.index * per) * BK;
-    const int ke = kb + per * BK;
-    u.kbeg = max(__builtin_amdgcn_readfirstlane(u.kbeg), kb);
-    u.kend = min(__builtin_amdgcn_readfirstlane(u.kend), ke);
-    // where the parts of this unit's rows are, for the merge
-    int *dir = f.prefix ? a.dir_prefix : a.dir_tail;
-    if (f.index == 0 && head == 0 && threadIdx.x == 0) {
-        dir[2 * u.run] = item;
-        dir[2 * u.run + 1] = f.chunks;
+    const long long slot0 = ((long long)item * a.n_kv_heads + head) * a.part_rows;
+    // where the parts of the rows are, for the merge: item, chunks, the first
+    // one's row (a prefix's: its block's first sequence)
+    int *dir = (f.prefix ? a.dir_prefix : a.dir_tail) + 4 * u.run;
+    if (f.alone) {
+        Tail s;
+        walk_tail<BF16>(a, head, u, lds + wave * 4096, 0, 1, lane, s);
+        if (f.chunks == 0) return;
+        const float l = col4_sum(s.l);
+        float *out = f.shares ? a.part_o + (slot0 + wave * a.group) * D : a.out + ((long long)u.run * a.n_kv_heads + head) * a.group * D;
+        if ((lane & 15) < a.group) {
+            store_tail_rows<BF16>(s, l > 0.f || l != l ? 1.0f / l : 0.f, out, lane);
+            if (f.shares && lane < 16) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * (slot0 + wave * a.group + lane)) = (f32x2){s.m, l};
+        }
+        if (head == 0 && lane == 0) *reinterpret_cast<u32x4 *>(dir) = (u32x4){(unsigned)item, 1, (unsigned)(wave * a.group), 0};
+        return;
+    }
+    if (f.index == 0 && head == 0 && (int)threadIdx.x < (f.prefix ? u.count / a.group : 1))
+        *reinterpret_cast<u32x4 *>(dir + 4 * threadIdx.x) =
+            (u32x4){(unsigned)item, (unsigned)f.chunks, f.prefix ? (unsigned)u.run : 0u, 0};
+    if (!f.prefix) {
+        Tail s;
+        walk_tail<BF16>(a, head, u, lds, wave, NW, lane, s);
+        // (an even share may leave the last chunk without keys: its part is empty)
+        const bool whole = f.chunks == 1 && !f.shares;
+        store_tail<BF16, NW>(a, s, lds, wave, lane,
+                             whole ? a.out + ((long long)u.run * a.n_kv_heads + head) * a.group * D : a.part_o + slot0 * D,
+                             whole ? nullptr : a.part_ml + slot0 * 2);
+        return;
     }
     Rows s;
     const int gs = __builtin_ctz(a.group);
@@ -1027,55 +1437,38 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_decode_kernel(g3k_paged
     begin_rows(s);
     walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, s);
     G3K_RECOMPUTE(lane);      // no output address is kept through the walk
-    int first;
-    const bool whole = !f.prefix && f.chunks == 1 && seq_prefix(a, u.b, first) == 0;
-    {
-        const int row = wave * 16 + (lane & 15);
-        float *out = nullptr, *ml = nullptr;
-        if (row < u.count) {
-            if (whole) {
-                out = a.out + ((long long)(u.run + (row >> gs)) * a.n_kv_heads * a.group + head * a.group +
-                               (row & (a.group - 1))) * D;
-            } else {
-                const long long slot = ((long long)item * a.n_kv_heads + head) * a.part_rows + row;
-                out = a.part_o + slot * D;
-                ml = a.part_ml + slot * 2;
-            }
-        }
-        store_row(s, out, ml, lane);
-    }
+    const int row = wave * 16 + (lane & 15);
+    const long long slot = slot0 + row;
+    store_row(s, row < u.count ? a.part_o + slot * D : nullptr, a.part_ml + slot * 2, lane);
 }
 
 // One wave per sequence and query head.
-template <int NW>
 __global__ __launch_bounds__(256) void paged_decode_merge_kernel(g3k_paged_args a) {
-    constexpr int ROWS = 16 * NW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = a.n_kv_heads * a.group;
     const long long id = (long long)blockIdx.x * 4 + wave;
     if (id >= (long long)a.s.num_seqs * heads) return;
     const int b = (int)(id / heads), h = (int)(id % heads);
     const int kvh = h / a.group, hg = h % a.group;
+    // (the directories are kept within the parts whatever they hold: a batch
+    // whose group bounds overlap leaves entries unwritten)
+    const u32x4 dt = *reinterpret_cast<const u32x4 *>(a.dir_tail + 4 * b);
+    u32x4 dp = {0, 0, 0, 0};
+    if (a.n_groups > 0) dp = *reinterpret_cast<const u32x4 *>(a.dir_prefix + 4 * b);
     int first;
     const int len = seq_len(a.s, b), p = seq_prefix(a, b, first);
-    const int tail = tiles_of(tail_begin(a, len, p), len) > 0;
-    // (kept within the parts whatever the directory holds: a batch whose group
-    // bounds overlap leaves entries unwritten)
-    const int at = tail ? clampi(a.dir_tail[2 * b], 0, a.items - 1) : 0;
-    const int chunks = tail ? clampi(a.dir_tail[2 * b + 1], 0, a.items - at) : 0;
-    if (p == 0 && chunks == 1) return;        // written by its one chunk
+    const bool tail = tiles_of(tail_begin(a, len, p), len) > 0;
+    if (p == 0 && tail && dt.y == 1) return;        // written by its one chunk
     const long long stride = (long long)a.n_kv_heads * a.part_rows;
     Joined j;
     j.clear();
-    const auto add = [&](long long slot, int n) {
+    const auto add = [&](u32x4 d, int row) {
+        const int item = clampi((int)d.x, 0, a.items - 1), n = clampi((int)d.y, 1, a.items - item);
+        const long long slot = ((long long)item * a.n_kv_heads + kvh) * a.part_rows + clampi(row, 0, a.part_rows - 1);
         for (int q = 0; q < n; q += 64) j.add(a, slot + (q + min(lane, n - 1 - q)) * stride, min(n - q, 64), lane);
     };
-    if (tail) add(((long long)at * a.n_kv_heads + kvh) * a.part_rows + hg, chunks);
-    if (p > 0) {
-        const int row = (b - first) * a.group + hg, lead = first + row / ROWS * (ROWS / a.group);
-        const int item = clampi(a.dir_prefix[2 * lead], 0, a.items - 1);
-        add(((long long)item * a.n_kv_heads + kvh) * a.part_rows + row % ROWS, clampi(a.dir_prefix[2 * lead + 1], 0, a.items - item));
-    }
+    if (tail) add(dt, (int)dt.z + hg);
+    if (p > 0) add(dp, (b - (int)dp.z) * a.group + hg);
     j.store(a.out + id * D, lane);
 }
 
@@ -1090,11 +1483,11 @@ void launch_prefill(const g3k_paged_args &a, unsigned wgs, hipStream_t st) {
     if (a.budget > 0) hipLaunchKernelGGL(paged_prefill_merge_kernel<NW>, dim3(merges), dim3(256), 0, st, a);
 }
 
-template <bool BF16, int NW>
+template <bool BF16>
 void launch_decode(const g3k_paged_args &a, unsigned wgs, hipStream_t st) {
-    hipLaunchKernelGGL((paged_decode_kernel<BF16, NW>), dim3(wgs), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL(paged_decode_kernel<BF16>, dim3(wgs), dim3(64 * DECODE_WAVES), 0, st, a);
     const unsigned merges = ((unsigned)a.s.num_seqs * a.n_kv_heads * a.group + 3) / 4;
-    hipLaunchKernelGGL(paged_decode_merge_kernel<NW>, dim3(merges), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(paged_decode_merge_kernel, dim3(merges), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -1113,7 +1506,6 @@ extern "C" int g3k_paged_decode(const g3k_paged_args *a, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     const long long wgs = (long long)a->items * a->n_kv_heads;
     if (wgs > INT_MAX || (long long)a->s.num_seqs * a->n_kv_heads * a->group > INT_MAX) return (int)hipErrorInvalidValue;
-    if (a->waves == 8) a->bf16 ? launch_decode<true, 8>(*a, (unsigned)wgs, st) : launch_decode<false, 8>(*a, (unsigned)wgs, st);
-    else a->bf16 ? launch_decode<true, 4>(*a, (unsigned)wgs, st) : launch_decode<false, 4>(*a, (unsigned)wgs, st);
+    a->bf16 ? launch_decode<true>(*a, (unsigned)wgs, st) : launch_decode<false>(*a, (unsigned)wgs, st);
     return (int)hipGetLastError();
 }

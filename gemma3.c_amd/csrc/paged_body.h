@@ -11,19 +11,15 @@ namespace g3k {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
-    return v;
-}
 
-// Sum over lanes 0..l.
-__device__ __forceinline__ int wave_scan_int(int v, int lane) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const int o = __shfl(v, lane >= m ? lane - m : lane);
-        v += lane >= m ? o : 0;
-    }
+// Sum over lanes 0..l: within rows of 16 lanes, then the rows' totals.
+__device__ __forceinline__ int wave_scan_int(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 to rows 2 and 3
     return v;
 }
 
@@ -48,6 +44,8 @@ __device__ __forceinline__ void seq_rows(const g3k_paged_seqs &s, int b, int &fi
     first = clampi(s.q_start[b], 0, s.total_q);
     n = clampi(s.q_start[b + 1], first, s.total_q) - first;
 }
+
+__device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_scan_int(v), 63); }
 
 }  // namespace g3k
 

@@ -289,7 +289,7 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(g3k_pages_args a) {
             c.copy = c.tail >= 0 && !(a.first[c.tail] == b && a.writers[c.tail] == a.ref[c.tail]);
             need = c.full - c.kept + c.copy;
         }
-        const int upto = wave_scan_int(need, lane);
+        const int upto = wave_scan_int(need);
         before = waves_before(__shfl(upto, 63), slot, wave, lane, total);
         c.offset = needed + before + upto - need;
         needed = total > INT_MAX - needed ? INT_MAX : needed + total;

@@ -2490,16 +2490,22 @@ int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pa
     g3k_paged_args a;
     fill_paged(c, layer, pages, batch, q, out, &a);
     const int Hkv = c->cfg.num_kv_heads;
-    a.waves = 8;
-    if ((long long)prefill_blocks(batch, c->group, 128) * Hkv < c->n_cu) a.waves = 4;
+    /* 128 rows a workgroup read the keys half as often as 64; where they
+     * leave CUs idle, 64 are quicker (9 prompts of 1 to 120 tokens: 23 us
+     * against 27; 5 chunks behind up to 9000 cached keys, bf16: 658 against
+     * 334). */
+    a.waves = (long long)prefill_blocks(batch, c->group, 128) * Hkv < c->n_cu ? 4 : 8;
     const int rows = 16 * a.waves;
     a.blocks = a.items = prefill_blocks(batch, c->group, rows);
     hipSetDevice(c->device);
     /* Where blocks are many their different lengths even out over the CUs;
-     * else the long ones' keys are cut. */
+     * else the long ones' keys are cut into two workgroups' worth a CU (fp32
+     * prompts, bf16 chunks: 456, 334 us; one a CU 443, 361; three 486, 336).
+     * Short keys are cut down to 2 tiles (the 9 short prompts: 23.1 us; down
+     * to 1, 23.6; to 4, 26). */
     if ((long long)a.blocks * Hkv <= 8LL * c->n_cu) {
-        a.budget = (3 * c->n_cu / 2 + Hkv - 1) / Hkv;
-        a.min_tiles = 8;
+        a.budget = (2 * c->n_cu + Hkv - 1) / Hkv;
+        a.min_tiles = 2;
         a.items = a.blocks + a.budget + 1;
         const size_t n = (size_t)a.items * Hkv * rows, ob = align256(n * D * sizeof(float));
         unsigned char *ws;
@@ -2529,23 +2535,27 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
         a.group_start = prefixes->group_start;
         a.prefix_len = prefixes->prefix_len;
     }
-    a.waves = a.n_groups && B * c->group > 64 * a.n_groups ? 8 : 4;
-    const int rows = 16 * a.waves;
-    /* items per KV head: one workgroup a CU, and one more for every run of
-     * keys (its last chunk is a part one) */
+    const int rows = G3K_PAGED_DECODE_ROWS;
+    /* Per KV head one chunk a CU, or as many as there are runs of keys (4 KV
+     * heads, 64 sequences behind 8192 keys: 55 us; 8 heads, 48 sequences in 3
+     * groups, bf16: 83; half as many as runs 53, 151; twice as many 81, 91);
+     * the last chunk of a run is a part one.  With more runs than CUs short sequences
+     * are one wave's work (same two: 106, 151 us if not). */
     const int units = B + (a.n_groups ? a.n_groups + B * c->group / rows : 0);
-    a.budget = units + (c->n_cu + Hkv - 1) / Hkv;
-    a.items = a.budget;
+    a.budget = (c->n_cu + Hkv - 1) / Hkv;
+    if (a.budget < units) a.budget = units;
+    a.pack = (long long)units * Hkv > c->n_cu;
+    a.items = a.budget + units;
     a.min_tiles = 2;
     a.part_rows = a.n_groups ? rows : c->group;
     const size_t n = (size_t)a.items * Hkv * a.part_rows, ob = align256(n * D * sizeof(float)), mb = align256(n * 2 * sizeof(float));
     hipSetDevice(c->device);
     unsigned char *ws;
-    PAGED_TRY(paged_scratch(c, ob + mb + (size_t)B * 4 * sizeof(int), fn, &ws));
+    PAGED_TRY(paged_scratch(c, ob + mb + (size_t)B * 8 * sizeof(int), fn, &ws));
     a.part_o = (float *)ws;
     a.part_ml = (float *)(ws + ob);
     a.dir_prefix = (int *)(ws + ob + mb);
-    a.dir_tail = a.dir_prefix + 2 * B;
+    a.dir_tail = a.dir_prefix + 4 * B;
     const int rc = g3k_paged_decode(&a, c->stream);
     if (rc) return hip_fail((hipError_t)rc, "g3attn_paged_decode launch");
     return G3_OK;

@@ -288,8 +288,11 @@ inline unsigned atomicInc(unsigned *p, unsigned v) {
 }
 
 // ---- cross-lane builtins ---------------------------------------------------------
-// DPP (row = 16 lanes): quad_perm 0x00-0xff, row_ror:8 0x128 (lane i reads
-// lane i ^ 8 of its row), row_mirror 0x140, row_half_mirror 0x141.
+// DPP (row = 16 lanes): quad_perm 0x00-0xff, row_shr:1-15 0x111-0x11f (lane i
+// reads lane i - n of its row; none: zero with bound_ctrl, else kept), row_ror:8
+// 0x128 (lane i reads lane i ^ 8 of its row), row_mirror 0x140,
+// row_half_mirror 0x141, row_bcast:15 0x142 (the last lane of the row before),
+// row_bcast:31 0x143 (lane 31, for rows 2 and 3).
 inline int hostemu_update_dpp(int old, int src, int ctrl, int row_mask, int bank_mask, bool bound_ctrl) {
     const int l = hostemu::t_lane;
     int from;
@@ -297,10 +300,16 @@ inline int hostemu_update_dpp(int old, int src, int ctrl, int row_mask, int bank
     else if (ctrl == 0x128) from = l ^ 8;
     else if (ctrl == 0x140) from = (l & ~15) + (15 - (l & 15));
     else if (ctrl == 0x141) from = (l & ~7) + (7 - (l & 7));
+    else if (ctrl >= 0x111 && ctrl <= 0x11f) from = (l & 15) - (ctrl & 15) >= 0 ? l - (ctrl & 15) : -1;
+    else if (ctrl == 0x142) from = l >= 16 ? (l & ~15) - 1 : -1;
+    else if (ctrl == 0x143) from = l >= 32 ? 31 : -1;
     else hostemu::fail("DPP control not emulated");
-    (void)bound_ctrl;
     uint32_t r, unused;
-    hostemu::exchange((uint32_t)src, 0, from, &r, &unused);
+    hostemu::exchange((uint32_t)src, 0, from < 0 ? l : from, &r, &unused);
+    if (from < 0) {
+        if (!bound_ctrl) return old;
+        r = 0;
+    }
     const bool enabled = ((row_mask >> (l >> 4)) & 1) && ((bank_mask >> ((l >> 2) & 3)) & 1);
     return enabled ? (int)r : old;
 }
@@ -518,6 +527,34 @@ inline F4 hostemu_mfma_16x16x32(V8 a, V8 b, F4 c, int cbsz, int abid, int blgp) 
 }
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16 hostemu_mfma_16x16x32
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 hostemu_mfma_16x16x32
+
+// V_MFMA_F32_16X16X16_F16: the same with a 16 x 16 A and B; lane l holds
+// A[l % 16][4 (l / 16) + j] and B[4 (l / 16) + j][l % 16], j < 4.
+template <typename V4, typename F4>
+inline F4 hostemu_mfma_16x16x16(V4 a, V4 b, F4 c, int cbsz, int abid, int blgp) {
+    static_assert(sizeof(V4) == 8, "4 x 16-bit operands");
+    if (cbsz || abid || blgp) hostemu::fail("MFMA broadcast controls not emulated");
+    hostemu::Wave &w = hostemu::machine()->waves[hostemu::t_wave];
+    const int l = hostemu::t_lane;
+    const int k = w.gen[l]++ & 1;
+    std::memcpy(&w.op[k][l][0], &a, 8);
+    std::memcpy(&w.op[k][l][4], &b, 8);
+    w.bar.wait();
+    const int n = l & 15, g = l >> 4;
+    F4 d;
+    for (int r = 0; r < 4; r++) {
+        double acc = (double)c[r];
+        for (int q = 0; q < 4; q++) {
+            V4 av, bv;
+            std::memcpy(&av, &w.op[k][4 * g + r + 16 * q][0], 8);
+            std::memcpy(&bv, &w.op[k][n + 16 * q][4], 8);
+            for (int j = 0; j < 4; j++) acc += (double)(float)av[j] * (double)(float)bv[j];
+        }
+        d[r] = (float)acc;
+    }
+    return d;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x16f16 hostemu_mfma_16x16x16
 
 // OCP fp8 e4m3 (FN: bias 7, no infinities, 0x7f / 0xff NaN, largest 448).
 inline float hostemu_e4m3_value(uint8_t b) {
