@@ -34,6 +34,11 @@
 // Hides where a lane's value comes from, so that what is computed from it is
 // computed again in every pass of a loop instead of being kept in registers
 // across it (no instruction).
+// A pointer's target is global memory.
+#ifndef G3K_GLOBAL
+#define G3K_GLOBAL __attribute__((address_space(1)))
+#endif
+
 #ifndef G3K_RECOMPUTE
 #define G3K_RECOMPUTE(x) asm volatile("" : "+v"(x))
 #endif

@@ -74,9 +74,26 @@ __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
 
 __device__ __forceinline__ half2v cvt2(float a, float b) { return __builtin_convertvector((f32x2){a, b}, half2v); }
 
+// The larger of two, NaN if either is (v_maximum3_f32: no canonicalising moves
+// before it, as before v_max_f32), and so over a row's lanes and the wave's.
+__device__ __forceinline__ float top(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float col4_top(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = top(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return top(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float wave_top(float v) {
+    v = top(v, dpp<0xB1>(v));      // within quads, their pairs, eights, sixteens
+    v = top(v, dpp<0x4E>(v));
+    v = top(v, dpp<0x141>(v));
+    v = top(v, dpp<0x140>(v));
+    return col4_top(v);
+}
+
 // The power-of-two exponent of a block whose largest magnitude is m: m <
 // 2^exponent.  A block of zeros, or of values below 2^-100, counts as 2^-100;
-// one with an infinity or NaN as 2^127 (its rows come out as they may).
+// one with an infinity or NaN as 2^127.
 __device__ __forceinline__ int block_exponent(float m) {
     if (!(m < INFINITY)) return 127;
     const int e = __builtin_amdgcn_frexp_expf(m);
@@ -125,9 +142,22 @@ struct Raw {
             return x[i];
         }
     }
+    __device__ __forceinline__ void set(int i, unsigned bits) {
+        if constexpr (BF16) x[i] = (u32x2){bits, bits};
+        else x[i] = (f32x4){__uint_as_float(bits), __uint_as_float(bits), __uint_as_float(bits), __uint_as_float(bits)};
+    }
 };
 
 __device__ const float zero_row[D] = {};
+
+// Pages and zero_row as what they are, global memory: through a generic
+// pointer their loads would count as LDS accesses too, and every wait for LDS,
+// barriers included, would be one for the rows in flight (packed prompts of
+// 8192 tokens: 514 us against 462).
+typedef const G3K_GLOBAL char *gbytes;
+template <class T>
+__device__ __forceinline__ T load_global(gbytes p) { return *reinterpret_cast<const G3K_GLOBAL T *>(p); }
+__device__ __forceinline__ gbytes global_bytes(const void *p) { return (gbytes)p; }
 
 // Where the rows of a walk are.  Looks pages up along it: 64 table entries in
 // a register, the next 64 on their way, so that a tile's lookup waits for no
@@ -186,15 +216,15 @@ struct Finder {
     // their run inside, so nothing else is read; their scores are masked.  A
     // page outside the pool is never followed, and neither is a run without a
     // key: the rows are zeros.
-    __device__ __forceinline__ void fetch(const char *matrix, const Place &p, int wave, int lane, Raw<BF16, NW> &raw) const {
+    __device__ __forceinline__ void fetch(gbytes matrix, const Place &p, int wave, int lane, Raw<BF16, NW> &raw) const {
         using T = typename std::conditional<BF16, u32x2, f32x4>::type;
         const int j0 = p.tile * BK;
         if (j0 >= kbeg && j0 + BK <= kend && !p.bad) {
 #pragma unroll
             for (int r = 0; r < RUNS; r++) {
-                const char *row = matrix + p.off[r] + 4 * (wave & 3) * ROW;
+                const gbytes row = matrix + p.off[r] + 4 * (wave & 3) * ROW;
 #pragma unroll
-                for (int i = 0; i < 4; i++) raw.x[4 * r + i] = *reinterpret_cast<const T *>(row + i * ROW + lane * (int)sizeof(T));
+                for (int i = 0; i < 4; i++) raw.x[4 * r + i] = load_global<T>(row + i * ROW + lane * (int)sizeof(T));
             }
             return;
         }
@@ -206,8 +236,8 @@ struct Finder {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int k = clampi(j + 4 * (wave & 3) + i, lo, hi) - j;
-                const char *row = none ? reinterpret_cast<const char *>(zero_row) : matrix + p.off[r] + k * ROW;
-                raw.x[4 * r + i] = *reinterpret_cast<const T *>(row + lane * (int)sizeof(T));
+                const gbytes row = none ? global_bytes(zero_row) : matrix + p.off[r] + k * ROW;
+                raw.x[4 * r + i] = load_global<T>(row + lane * (int)sizeof(T));
             }
         }
     }
@@ -220,10 +250,34 @@ __device__ __forceinline__ float rows_max(const Raw<BF16, NW> &raw) {
 #pragma unroll
     for (int i = 0; i < 4 * Raw<BF16, NW>::RUNS; i++) {
         const f32x4 x = raw.get(i);
-        m = fmaxf(fmaxf(m, fabsf(x.x)), fabsf(x.y));
-        m = fmaxf(fmaxf(m, fabsf(x.z)), fabsf(x.w));
+        m = top(top(m, fabsf(x.x)), fabsf(x.y));
+        m = top(top(m, fabsf(x.z)), fabsf(x.w));
     }
     return m;
+}
+
+// The largest finite magnitude of this wave's rows in flight, where some hold
+// an infinity or a NaN (seldom any): those rows, one bit each in `spoiled`, are
+// left out of the exponent, which is their neighbours' too.  K's become NaN,
+// and so their scores, which are masked for the rows that do not see them.
+// V's become zeros, since a value that is not finite times p = 0 is NaN in
+// every row of the product; a row that sees the key is made NaN instead.
+template <bool KEYS, bool BF16, int NW>
+__device__ __forceinline__ float settle(Raw<BF16, NW> &raw, int &spoiled) {
+    spoiled = 0;
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4 * Raw<BF16, NW>::RUNS; i++) {
+        const f32x4 x = raw.get(i);
+        const float y = top(top(fabsf(x.x), fabsf(x.y)), top(fabsf(x.z), fabsf(x.w)));
+        if (__builtin_amdgcn_ballot_w64(!(y < INFINITY))) {
+            spoiled |= 1 << i;
+            raw.set(i, KEYS ? BF16 ? 0x7fc07fc0u : 0x7fc00000u : 0u);
+        } else {
+            most = top(most, y);
+        }
+    }
+    return wave_top(most);
 }
 
 // K's rows (exponent e over the wave) as operands: lane holds dims 4 lane.. = half (lane & 1) of operand
@@ -264,14 +318,16 @@ __device__ __forceinline__ void store_k(const Raw<BF16, NW> &raw, int e, int bad
 
 // V's rows as operands: lane holds dims 4 lane + t of operand lane lane & 15 of
 // group g of dim blocks 4 (lane >> 4) + t, its keys 4 c.. of the operand's 8.
+// exps[run][group]: the exponent of these keys in 12 bits, above them one bit
+// for each spoiled key.
 template <bool BF16, int NW>
-__device__ __forceinline__ void store_v(const Raw<BF16, NW> &raw, int e, char *buf, int *exps, int wave, int lane) {
+__device__ __forceinline__ void store_v(const Raw<BF16, NW> &raw, int e, int spoiled, char *buf, int *exps, int wave, int lane) {
     using L = Lds<BF16>;
     constexpr int N = 4 * Raw<BF16, NW>::RUNS;
     typedef _Float16 Keys __attribute__((ext_vector_type(N)));
     const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
     const int c = NW == 4 ? 0 : wave >> 2;
-    if (lane < 8 / NW) exps[4 * (NW == 4 ? lane : c) + (wave & 3)] = e;
+    if (lane < 8 / NW) exps[4 * (NW == 4 ? lane : c) + (wave & 3)] = e + ((spoiled >> 4 * lane & 15) << 12);
     char *vd = buf + (lane >> 4) * (4 * L::PL * 1024) + (wave & 3) * 256 + (lane & 15) * 16 + c * 8;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -318,10 +374,10 @@ __device__ __forceinline__ void load_query(const float *q, bool live, float qsca
         for (int i = 0; i < 4; i++) {
             x[kk][i] = a[i];
             x[kk][4 + i] = b[i];
-            m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            m = top(top(m, fabsf(a[i])), fabsf(b[i]));
         }
     }
-    const int e = block_exponent(col4_max(m));
+    const int e = block_exponent(col4_top(m));
     const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
     s.factor = __builtin_amdgcn_ldexpf(qscale, e - X_EXP);
 #pragma unroll
@@ -374,9 +430,12 @@ __device__ __forceinline__ void tile_scores(const char *buf, int lane, const Row
 
 // Scores to probabilities (in place), the running max and sum, and O^T's
 // rescaling, which is rare: a row's max moves only when a score outgrows it by
-// 2^LAZY.  fac[run]: the factor and mask of this lane group's keys.
-__device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, int lane, Rows &s, f32x4 (&sc)[2]) {
-    const int j0 = tile * BK, g = lane >> 4;
+// 2^LAZY.  fac[run]: the factor and mask of this lane group's keys.  other()
+// is called if `also`, in the same branch: one branch more costs 4 to 10% of
+// the whole, since nothing is scheduled across it.
+template <class Other>
+__device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, int lane, Rows &s, f32x4 (&sc)[2], bool also, Other other) {
+    const int j0 = tile * BK;
     const bool ragged = j0 < s.lo_max || j0 + BK > s.hi_min;
     float t = M_NONE;
 #pragma unroll
@@ -386,27 +445,29 @@ __device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, in
         for (int r = 0; r < 4; r++) sc[kt][r] = __builtin_fmaf(sc[kt][r], f, fac[kt].y);
     }
     if (ragged) {
+        G3K_RECOMPUTE(lane);      // (what follows is not done ahead of the branch)
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int j = j0 + 16 * kt + 4 * g + r;
+                const int j = j0 + 16 * kt + 4 * (lane >> 4) + r;
                 if (j < s.lo || j >= s.hi) sc[kt][r] = -INFINITY;
             }
     }
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) t = fmaxf(t, sc[kt][r]);
-    t = col4_max(t);
+        for (int r = 0; r < 4; r++) t = top(t, sc[kt][r]);
+    t = col4_top(t);
     const bool up = t > s.m + LAZY;
-    if (__builtin_amdgcn_ballot_w64(up)) {
+    if (__builtin_amdgcn_ballot_w64(up || also)) {
         const float m = up ? t : s.m;
         const float keep = fast_exp2(s.m - m);
         s.m = m;
         s.l *= keep;
 #pragma unroll
         for (int d = 0; d < 16; d++) s.o[d] *= keep;
+        if (__builtin_amdgcn_ballot_w64(also)) other();
     }
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
@@ -417,23 +478,42 @@ __device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, in
         }
 }
 
-// P as the operand of P.V, scaled by its keys' V exponent against O^T's.  The
-// one O^T is held at is two bits above what the first tile has, so ordinary
-// tiles do not move it.
-__device__ __forceinline__ void split_p(const f32x4 (&p)[2], const int *exps, int lane, Rows &s, half8 &ph, half8 &pl) {
+// P of a tile as the operand of P.V, scaled by its keys' V exponent against
+// O^T's.  The one O^T is held at is two bits above what the first tile has, so
+// ordinary tiles do not move it.
+__device__ __forceinline__ int exponent_of(int packed) { return (int)((unsigned)packed << 20) >> 20; }
+__device__ __forceinline__ void split_p(const f32x4 (&p)[2], const int *exps, int tile, int lane, Rows &s, half8 &ph, half8 &pl) {
+    const int mine[2] = {exps[lane >> 4], exps[4 + (lane >> 4)]};
     int most = exps[0];
 #pragma unroll
     for (int i = 1; i < 8; i++) most = max(most, exps[i]);
-    const int top = __builtin_amdgcn_readfirstlane(most);
-    if (top > s.ev) {
-        const float down = s.ev == E_NONE ? 0.f : __builtin_amdgcn_ldexpf(1.0f, s.ev - top - 2);
-        s.ev = top + 2;
+    int up = __builtin_amdgcn_readfirstlane(most);
+    if (up > s.ev) {
+        if (up >= 1 << 11) {         // keys are spoiled
+            G3K_RECOMPUTE(lane);
+            G3K_RECOMPUTE(exps);
+            most = exponent_of(exps[0]);
 #pragma unroll
-        for (int d = 0; d < 16; d++) s.o[d] *= down;
+            for (int i = 1; i < 8; i++) most = max(most, exponent_of(exps[i]));
+            up = __builtin_amdgcn_readfirstlane(most);
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = tile * BK + 16 * kt + 4 * (lane >> 4) + r;
+                    if (((mine[kt] - exponent_of(mine[kt])) >> (12 + r) & 1) && j >= s.lo && j < s.hi) s.l = NAN;
+                }
+        }
+        if (up > s.ev) {
+            const float down = s.ev == E_NONE ? 0.f : __builtin_amdgcn_ldexpf(1.0f, s.ev - up - 2);
+            s.ev = up + 2;
+#pragma unroll
+            for (int d = 0; d < 16; d++) s.o[d] *= down;
+        }
     }
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
-        const float f = __builtin_amdgcn_ldexpf(1.0f, P_EXP + exps[4 * kt + (lane >> 4)] - s.ev);
+        const float f = __builtin_amdgcn_ldexpf(1.0f, P_EXP + exponent_of(mine[kt]) - s.ev);
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
             half2v h, l;
@@ -489,7 +569,7 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
     if (n <= 0) return;
     char *kbuf = lds, *vbuf = lds + 2 * L::K_BYTES;
     const long long head_off = ((long long)head << a.s.page_shift) * D * (BF16 ? 2 : 4);
-    const char *kb = static_cast<const char *>(a.k) + head_off, *vb = static_cast<const char *>(a.v) + head_off;
+    const gbytes kb = global_bytes(a.k) + head_off, vb = global_bytes(a.v) + head_off;
     Finder<BF16, NW> find;
     find.begin(a, u, lane);
     Raw<BF16, NW> rk, rv;
@@ -505,18 +585,19 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         pk = find.place(t0 + min(ik, n - 1), wave, lane);
         find.fetch(kb, pk, wave, lane, rk);
     };
-    const auto next_v = [&](int e) {
-        store_v<BF16, NW>(rv, e, vbuf + (iv & 1) * L::V_BYTES, exps + 8 * (iv & 1), wave, lane);
+    const auto next_v = [&](int e, int spoiled) {
+        store_v<BF16, NW>(rv, e, spoiled, vbuf + (iv & 1) * L::V_BYTES, exps + 8 * (iv & 1), wave, lane);
         iv++;
         find.fetch(vb, pv, wave, lane, rv);
     };
     const int lead = NW == 8 ? wave >> 2 : 0;
-    const auto exponent = [&](const Raw<BF16, NW> &r) { return block_exponent(wave_max(rows_max<BF16, NW>(r))); };
-    next_k(exponent(rk));
+    int spoiled;
+    next_k(block_exponent(settle<true>(rk, spoiled)));
     if (lead) {
         pv = pk;
-        next_v(exponent(rv));
-        next_k(exponent(rk));
+        const int ev = block_exponent(settle<false>(rv, spoiled));
+        next_v(ev, spoiled);
+        next_k(block_exponent(settle<true>(rk, spoiled)));
     }
     // only LDS has to have arrived at these barriers: 63 vector memory
     // operations may stay in flight
@@ -533,7 +614,7 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         const f32x2 fac[2] = {f[0], f[4]};
         tile_scores<BF16>(kbuf + x * L::K_BYTES, lane, s, sc);
         if (i > 0) {
-            split_p(p, exps + 8 * (x ^ 1), lane, s, ph, pl);
+            split_p(p, exps + 8 * (x ^ 1), t - 1, lane, s, ph, pl);
             tile_values<BF16>(vbuf + (x ^ 1) * L::V_BYTES, lane, ph, pl, s);
         }
         p[0] = sc[0];
@@ -541,13 +622,17 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         if (NW == 8) G3K_WAIT_BARRIER(63);
         // V(i - 1)
         // (three chains of cross-lane steps side by side)
-        const int ek = exponent(rk), ev = exponent(rv);
-        tile_softmax(fac, t, lane, s, p);
-        next_k(ek);
-        next_v(ev);
+        float mk = wave_top(rows_max<BF16, NW>(rk)), mv = wave_top(rows_max<BF16, NW>(rv));
+        spoiled = 0;
+        tile_softmax(fac, t, lane, s, p, !(top(mk, mv) < INFINITY), [&]() {
+            mk = settle<true>(rk, spoiled);
+            mv = settle<false>(rv, spoiled);
+        });
+        next_k(block_exponent(mk));
+        next_v(block_exponent(mv), spoiled);
         G3K_WAIT_BARRIER(63);
     }
-    split_p(p, exps + 8 * ((n - 1) & 1), lane, s, ph, pl);
+    split_p(p, exps + 8 * ((n - 1) & 1), t0 + n - 1, lane, s, ph, pl);
     tile_values<BF16>(vbuf + ((n - 1) & 1) * L::V_BYTES, lane, ph, pl, s);
     // the second four are a phase behind: one barrier more before, one less after
     if (NW == 8 && !lead) G3K_WAIT_BARRIER(63);
@@ -786,11 +871,11 @@ struct Joined {
             pl = st.y;
         }
         fetch(0);
-        const float top = fmaxf(wave_max(pm), m);
-        const float w = pl * fast_exp2(pm - top), keep = fast_exp2(m - top);
+        const float most = top(wave_top(pm), m);
+        const float w = pl * fast_exp2(pm - most), keep = fast_exp2(m - most);
         o *= keep;
         l = l * keep + wave_sum(w);
-        m = top;
+        m = most;
         for (int i0 = 0;;) {
 #pragma unroll
             for (int i = 0; i < AT; i++)
@@ -1080,17 +1165,17 @@ struct Step {
     u32x4 k[N], v[N];
     // Lane (c, g)'s offsets from the step's first row; rows outside [0, rows)
     // of it are the nearest one's.
-    __device__ __forceinline__ void load_k(const char *base, int rs, int first, int end, int lane) {
-        const char *row = base + clampi(lane & 15, first, end - 1) * rs + (lane >> 4) * 16;
+    __device__ __forceinline__ void load_k(gbytes base, int rs, int first, int end, int lane) {
+        const gbytes row = base + clampi(lane & 15, first, end - 1) * rs + (lane >> 4) * 16;
 #pragma unroll
-        for (int i = 0; i < N; i++) k[i] = *reinterpret_cast<const u32x4 *>(row + i * 64);
+        for (int i = 0; i < N; i++) k[i] = load_global<u32x4>(row + i * 64);
     }
-    __device__ __forceinline__ void load_v(const char *base, int rs, int first, int end, int lane) {
+    __device__ __forceinline__ void load_v(gbytes base, int rs, int first, int end, int lane) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const char *row = base + clampi(4 * (lane >> 4) + i, first, end - 1) * rs + (lane & 15) * 16;
+            const gbytes row = base + clampi(4 * (lane >> 4) + i, first, end - 1) * rs + (lane & 15) * 16;
 #pragma unroll
-            for (int T = 0; T < N / 4; T++) v[T * 4 + i] = *reinterpret_cast<const u32x4 *>(row + T * 256);
+            for (int T = 0; T < N / 4; T++) v[T * 4 + i] = load_global<u32x4>(row + T * 256);
         }
     }
 };
@@ -1108,9 +1193,9 @@ __device__ __forceinline__ float step_max(const u32x4 (&x)[BF16 ? 8 : 16]) {
     for (int i = 0; i < (BF16 ? 8 : 16); i++)
 #pragma unroll
         for (int e = 0; e < (BF16 ? 8 : 4); e += 2)
-            m = BF16 ? fmaxf(fmaxf(m, fabsf(bf16_of(x[i], e))), fabsf(bf16_of(x[i], e + 1)))
-                     : fmaxf(fmaxf(m, fabsf(f32_of(x[i], e))), fabsf(f32_of(x[i], e + 1)));
-    return wave_max(m);
+            m = BF16 ? top(top(m, fabsf(bf16_of(x[i], e))), fabsf(bf16_of(x[i], e + 1)))
+                     : top(top(m, fabsf(f32_of(x[i], e))), fabsf(f32_of(x[i], e + 1)));
+    return wave_top(m);
 }
 
 // The dim of element i of dim step kk's operand lane of group g: K's loads are
@@ -1144,7 +1229,7 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
     const int *table = a.s.page_table + (long long)u.b * a.s.table_stride;
     const int shift = a.s.page_shift, mask = (1 << shift) - 1, last = max(u.kend - 1, 0) >> shift;
     const long long head_off = ((long long)head << shift) * D;
-    const char *kb = static_cast<const char *>(a.k) + head_off * (ROW / D), *vb = static_cast<const char *>(a.v) + head_off * (ROW / D);
+    const gbytes kb = global_bytes(a.k) + head_off * (ROW / D), vb = global_bytes(a.v) + head_off * (ROW / D);
     // lane i: the page of this wave's step base + i
     const auto look = [&](int base) { return table[min((j0 + 16 * (step0 + stride * (base + lane))) >> shift, last)]; };
     int ids = look(0);
@@ -1178,7 +1263,7 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
     const int mine = steps > step0 ? (steps - step0 + stride - 1) / stride : 0;
     const auto begin = [&](int n) { return max(u.kbeg - (j0 + 16 * (step0 + stride * n)), 0); };
     const auto end = [&](int n) { return min(u.kend - (j0 + 16 * (step0 + stride * n)), 16); };
-    const char *zeros = reinterpret_cast<const char *>(zero_row);
+    const gbytes zeros = global_bytes(zero_row);
     Where w = {0, 0};
     if (mine > 0) {
         w = where(0);
@@ -1191,8 +1276,8 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
 #pragma unroll
         for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(xq[kk][i >> 2][i & 3]));
-        const int e = block_exponent(col4_max(m));
+            for (int i = 0; i < 8; i++) m = top(m, fabsf(xq[kk][i >> 2][i & 3]));
+        const int e = block_exponent(col4_top(m));
         const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
         qfac = __builtin_amdgcn_ldexpf(a.qscale, e - X_EXP);
 #pragma unroll
@@ -1217,7 +1302,8 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
         const int first = begin(n), fin = end(n);
         const bool gone = w.rs == 0;
         G3K_RECOMPUTE(lane);
-        const int ek = block_exponent(step_max<BF16>(x.k));
+        const float mk = step_max<BF16>(x.k);
+        const int ek = block_exponent(mk);
         const float sk = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ek);
         f32x4 sc = {0.f, 0.f, 0.f, 0.f}, sx = sc, sy = sc;
         const char *qp = queries + (4 * (lane >> 4) + (lane & 3)) * 16;
@@ -1256,10 +1342,12 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
         for (int r = 0; r < 4; r++) {
             const int j = 4 * g + r;
             sc[r] = gone || j < first || j >= fin ? -INFINITY : sc[r] * f;
-            t = fmaxf(t, sc[r]);
+            t = top(t, sc[r]);
         }
-        t = col4_max(t);
-        const int ev = block_exponent(step_max<BF16>(x.v));
+        t = col4_top(t);
+        const float mv = step_max<BF16>(x.v);
+        if (!(mk < INFINITY) || !(mv < INFINITY)) s.l = NAN;     // every head sees the step's rows
+        const int ev = block_exponent(mv);
         const bool up = t > s.m + LAZY;
         if (__builtin_amdgcn_ballot_w64(up) || ev > s.ev) {
             const float m = up ? t : s.m;
@@ -1356,21 +1444,21 @@ __device__ __forceinline__ void store_tail(const g3k_paged_args &a, Tail &s, cha
     __syncthreads();
     for (int i = threadIdx.x; i < a.group * (D / 4); i += 64 * NW) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
-        float top = M_NONE;
+        float most = M_NONE;
 #pragma unroll
-        for (int w = 0; w < NW; w++) top = fmaxf(top, st[2 * (w * 4 + row)]);
+        for (int w = 0; w < NW; w++) most = top(most, st[2 * (w * 4 + row)]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float k = st[2 * (w * 4 + row) + 1] * fast_exp2(st[2 * (w * 4 + row)] - top);
+            const float k = st[2 * (w * 4 + row) + 1] * fast_exp2(st[2 * (w * 4 + row)] - most);
             sum += k;
             o += k * *reinterpret_cast<const f32x4 *>(ws + (w * 4 + row) * D + d);
         }
         const float y = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
         *reinterpret_cast<f32x4 *>(out + row * D + d) = o * y;
         if (ml && d == 0) {
-            ml[2 * row] = top;
+            ml[2 * row] = most;
             ml[2 * row + 1] = sum;
         }
     }

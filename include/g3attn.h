@@ -434,10 +434,12 @@ int g3attn_paged_write_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pa
  * keys included (written before): q as g3attn_paged_write_device leaves it,
  * out [total_q][num_heads * 256].  The token at position p sees positions
  * [0, p], or [p - sliding_window + 1, p] on a local layer.  A token that sees
- * no key gets zeros.  Scores and products hold 22 bits of q, K, V and the
- * probabilities, with fp32 sums: about 3e-7 of the output's RMS (keys that
- * are seen have to be finite).  The result does not depend on what else is in
- * the batch beyond the order of sums. */
+ * no key gets zeros; one that sees a key or value with an infinity or a NaN
+ * in it gives NaN, and no other one does.  Scores and products hold 22 bits of
+ * q, K, V and the probabilities, with fp32 sums: about 3e-7 of the output's
+ * RMS.  (The bits of a small element count from the largest magnitude among
+ * 16 of the head's rows: 2^-38 of it are lost.)  The result does not depend on
+ * what else is in the batch beyond the order of sums. */
 int g3attn_paged_prefill_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pages, const g3attn_batch *batch,
                                 const float *q, float *out);
 

@@ -49,6 +49,7 @@
 //   paged_decode layer slot num_groups group_start|- prefix_len|- q out
 //   pages_fork from parent|- add|- held|- to status     (slots)
 //   pages_compact from held|- to status
+//   paged_refusals                                              (4 heads over 2, 6 layers)
 //                    (all of these with device copies; outputs hold what the
 //                    named file holds before the call where it exists)
 //   front_stage_only Hkv nk V vt_out            (g3k_rope_write_stage with an
@@ -191,6 +192,112 @@ void check(int rc, const std::string &call) {
     }
 }
 
+// Every argument that the host can refuse, one at a time: a code, a message,
+// and nothing touched (the pointers lead nowhere).
+int paged_refusals(g3attn_ctx *ctx) {
+    char *const A = reinterpret_cast<char *>(1ull << 40);
+    const long long rows = 2 * 16 * 256;
+    const g3attn_pages pages{A, A, G3ATTN_PAGE_F32, 0, 6, 8, 16, rows, 8 * rows};
+    const g3attn_seqs seqs{2, (int *)A, (int *)A, 4};
+    const g3attn_batch packed{seqs, 7, (int *)A}, single{seqs, 2, nullptr};
+    const float *F = (const float *)A;
+    float *O = (float *)A;
+    const uint16_t *N = (const uint16_t *)A;
+    int calls = 0;
+    const auto refused = [&](int rc, const char *what) {
+        calls++;
+        if (rc != -1 || !*g3attn_last_error()) {
+            std::fprintf(stderr, "attn_emu: %s was not refused (%d)\n", what, rc);
+            std::exit(1);
+        }
+    };
+    const auto with_pages = [&](int layer, const g3attn_pages *p, const char *what) {
+        refused(g3attn_paged_write_device(ctx, layer, p, &packed, F, F, F, nullptr, nullptr, O), what);
+        refused(g3attn_paged_prefill_device(ctx, layer, p, &packed, F, O), what);
+        refused(g3attn_paged_decode_device(ctx, layer, p, &single, nullptr, F, O), what);
+    };
+    const auto bad_page = [&](const char *what, auto change) {
+        g3attn_pages p = pages;
+        change(p);
+        with_pages(0, &p, what);
+        refused(g3attn_pages_fork_device(ctx, &p, &seqs, nullptr, nullptr, nullptr, &seqs, nullptr), what);
+        refused(g3attn_pages_compact_device(ctx, &p, &seqs, nullptr, &seqs, nullptr), what);
+    };
+    bad_page("null k", [](g3attn_pages &p) { p.k = nullptr; });
+    bad_page("null v", [](g3attn_pages &p) { p.v = nullptr; });
+    bad_page("k off 16 bytes", [](g3attn_pages &p) { p.k = (char *)p.k + 4; });
+    bad_page("v off 16 bytes", [](g3attn_pages &p) { p.v = (char *)p.v + 8; });
+    for (int x : {-1, 2}) bad_page("dtype", [&](g3attn_pages &p) { p.dtype = x; });
+    for (int x : {-16, 0, 8, 24, 2048}) bad_page("page_size", [&](g3attn_pages &p) { p.page_size = x; });
+    for (int x : {-1, 0}) bad_page("num_pages", [&](g3attn_pages &p) { p.num_pages = x; });
+    for (int x : {-1, 0, 4097}) bad_page("num_layers", [&](g3attn_pages &p) { p.num_layers = x; });
+    bad_page("first_layer", [](g3attn_pages &p) { p.first_layer = -1; });
+    for (long long x : {0ll, rows - 8, rows + 4, -rows, (1ll << 31) + 8}) bad_page("page_stride", [&](g3attn_pages &p) { p.page_stride = x; });
+    for (long long x : {0ll, 8ll, 7 * rows, 8 * rows + 4}) bad_page("layer_stride", [&](g3attn_pages &p) { p.layer_stride = x; });
+    for (int layer : {-1, 6}) with_pages(layer, &pages, "layer");
+    g3attn_pages later = pages;
+    later.first_layer = 1;
+    with_pages(0, &later, "layer before the pool's");
+    later.first_layer = 0;
+    later.num_layers = 5;
+    with_pages(5, &later, "layer behind the pool's");
+    with_pages(0, nullptr, "null pages");
+
+    const auto bad_seqs = [&](const char *what, auto change) {
+        g3attn_seqs x = seqs;
+        change(x);
+        const g3attn_batch pk{x, 7, (int *)A}, sg{x, x.num_seqs, nullptr};
+        refused(g3attn_paged_write_device(ctx, 0, &pages, &pk, F, F, F, nullptr, nullptr, O), what);
+        refused(g3attn_paged_prefill_device(ctx, 0, &pages, &pk, F, O), what);
+        refused(g3attn_paged_decode_device(ctx, 0, &pages, &sg, nullptr, F, O), what);
+        refused(g3attn_pages_fork_device(ctx, &pages, &x, nullptr, nullptr, nullptr, &seqs, nullptr), what);
+        refused(g3attn_pages_fork_device(ctx, &pages, &seqs, nullptr, nullptr, nullptr, &x, nullptr), what);
+        refused(g3attn_pages_compact_device(ctx, &pages, &seqs, nullptr, &x, nullptr), what);
+        refused(g3attn_pages_compact_device(ctx, &pages, &x, nullptr, &seqs, nullptr), what);
+    };
+    for (int x : {-1, 0, 4097}) bad_seqs("num_seqs", [&](g3attn_seqs &q) { q.num_seqs = x; });
+    bad_seqs("kv_len", [](g3attn_seqs &q) { q.kv_len = nullptr; });
+    bad_seqs("page_table", [](g3attn_seqs &q) { q.page_table = nullptr; });
+    for (int x : {-1, 0, (1 << 20) + 1}) bad_seqs("table_stride", [&](g3attn_seqs &q) { q.table_stride = x; });
+    g3attn_seqs wide = seqs, more = seqs;
+    wide.table_stride = 5;
+    more.num_seqs = 3;
+    refused(g3attn_pages_fork_device(ctx, &pages, &seqs, nullptr, nullptr, nullptr, &wide, nullptr), "two table strides");
+    refused(g3attn_pages_compact_device(ctx, &pages, &seqs, nullptr, &wide, nullptr), "two table strides");
+    refused(g3attn_pages_compact_device(ctx, &pages, &seqs, nullptr, &more, nullptr), "two numbers of sequences");
+
+    for (int n : {-1, (1 << 24) + 1}) {
+        const g3attn_batch b{seqs, n, (int *)A};
+        refused(g3attn_paged_write_device(ctx, 0, &pages, &b, F, F, F, nullptr, nullptr, O), "total_q");
+        refused(g3attn_paged_prefill_device(ctx, 0, &pages, &b, F, O), "total_q");
+    }
+    const g3attn_batch three{seqs, 3, nullptr};
+    refused(g3attn_paged_prefill_device(ctx, 0, &pages, &three, F, O), "total_q without q_start");
+    refused(g3attn_paged_prefill_device(ctx, 0, &pages, nullptr, F, O), "null batch");
+    refused(g3attn_paged_decode_device(ctx, 0, &pages, &packed, nullptr, F, O), "decode of packed rows");
+    for (int i = 0; i < 4; i++)
+        for (const char *x : {(const char *)nullptr, (const char *)A + 4}) {
+            const float *a[4] = {F, F, F, F};
+            a[i] = (const float *)x;
+            refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, a[0], a[1], a[2], nullptr, nullptr, (float *)a[3]), "write buffers");
+            if (i > 1) continue;
+            refused(g3attn_paged_prefill_device(ctx, 0, &pages, &packed, a[0], (float *)a[1]), "prefill buffers");
+            refused(g3attn_paged_decode_device(ctx, 0, &pages, &single, nullptr, a[0], (float *)a[1]), "decode buffers");
+        }
+    refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, N, nullptr, O), "q_norm alone");
+    refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, nullptr, N, O), "k_norm alone");
+    refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, N, (const uint16_t *)(A + 2), O), "k_norm alignment");
+    for (const g3attn_prefixes &p : {g3attn_prefixes{-1, (int *)A, (int *)A}, g3attn_prefixes{3, (int *)A, (int *)A},
+                                     g3attn_prefixes{1, nullptr, (int *)A}, g3attn_prefixes{1, (int *)A, nullptr}})
+        refused(g3attn_paged_decode_device(ctx, 0, &pages, &single, &p, F, O), "prefixes");
+    refused(g3attn_paged_write_device(nullptr, 0, &pages, &packed, F, F, F, nullptr, nullptr, O), "null context");
+    refused(g3attn_paged_prefill_device(nullptr, 0, &pages, &packed, F, O), "null context");
+    refused(g3attn_paged_decode_device(nullptr, 0, &pages, &single, nullptr, F, O), "null context");
+    refused(g3attn_pages_fork_device(nullptr, &pages, &seqs, nullptr, nullptr, nullptr, &seqs, nullptr), "null context");
+    refused(g3attn_pages_compact_device(nullptr, &pages, &seqs, nullptr, &seqs, nullptr), "null context");
+    return calls;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -317,6 +424,8 @@ int main(int argc, char **argv) {
                 check(g3attn_pages_compact_device(ctx, &paged.pages, &paged.seqs[from], held, &paged.seqs[to], status), cmd);
             }
             write_bin(sf, status, 2);
+        } else if (cmd == "paged_refusals") {
+            std::printf("attn_emu: refused %d calls\n", paged_refusals(ctx));
         } else if (cmd == "kv_write" || cmd == "kv_read") {
             int layer, slot, n;
             std::string kf, vf;

@@ -586,3 +586,163 @@ def run_compact(r, lens, ps, pages, bf16=False, held=None, seed=0, alias=False, 
 
 def _same(got, want, label):
     assert np.array_equal(np.asarray(got), np.asarray(want)), f"{label}: {got} is not {want}"
+
+
+# ------------------------------------------------------------------ harder cases
+
+def run_spoiled(r, layer, ps, bf16, spots, q_lens=None, lens=None, members=None, prefix=None, tail=None, seed=0, label="spoiled"):
+    """Infinities and NaN in single elements of keys and values that some rows
+    see: spots are (sequence, position, "k" or "v", value).  Rows that see one
+    are NaN, all others as they are without."""
+    rng = np.random.default_rng(seed)
+    prompts = q_lens is not None
+    if not prompts:
+        group = [i for i, m in enumerate(members) for _ in range(m)]
+        lens = [prefix[group[i]] + t for i, t in enumerate(tail)]
+    first = np.concatenate([[0], np.cumsum(members if members else [len(lens)])])
+    shared = [] if prompts else [(int(first[i]), m, prefix[i] // ps) for i, m in enumerate(members)]
+    assert prompts or all(p % ps == 0 for p in prefix)      # a prefix is whole pages here
+    table = tables_for(rng, lens, ps, sum(-(-n // ps) for n in lens) + 2, shared=shared)
+    pool = Pool(rng, 1, int(table.max()) + 2, r.hkv, ps, bf16, first_layer=layer)
+    pool.fill(rng, table, lens)
+    start = np.concatenate([[0], np.cumsum(q_lens)]) if prompts else np.arange(len(lens) + 1)
+    q = (rng.standard_normal((int(start[-1]), r.hq, D)) * 2).astype(np.float32)
+    want = packed_attention(pool, layer, r.span(layer), table, lens, start, q)
+    lost = np.zeros(want.shape[:2], bool)                   # [row][head]
+    for i, (b, j, which, value) in enumerate(spots):
+        h = i % r.hkv
+        page = table[b, j // ps]
+        getattr(pool, which)[0, page, h, j % ps, (37 * i + 5) % D] = value
+        for s in range(len(lens)):
+            if j // ps < table.shape[1] and table[s, j // ps] == page and j < lens[s]:
+                n = start[s + 1] - start[s]
+                for t in range(n):
+                    pos = lens[s] - n + t
+                    if j <= pos and j > pos - r.span(layer):
+                        lost[start[s] + t, h * r.hq // r.hkv:(h + 1) * r.hq // r.hkv] = True
+    assert lost.any() and not lost.all()
+
+    def check(out):
+        assert np.isnan(out[lost]).all(), f"{label}: a row that sees a spoiled key is not NaN"
+        check_close(out[~lost], want[~lost], label)
+    r.pool(pool)
+    r.seqs(0, lens, table)
+    if prompts:
+        r.prefill(layer, 0, start, q, check)
+    else:
+        r.decode(layer, 0, (first, prefix), q, check)
+
+
+SPOTS = [(0, 3, "v", np.nan), (0, 30, "k", np.inf), (0, 33, "v", -np.inf), (1, 40, "k", np.nan), (1, 61, "v", np.inf)]
+
+
+def run_spoiled_all(r, layer, bf16):
+    """Rows before a spoiled key, behind a window, in other heads and sequences."""
+    run_spoiled(r, layer, 16, bf16, SPOTS, q_lens=[70, 25, 20], lens=[70, 77, 20], label="spoiled prompts")
+    run_spoiled(r, layer, 16, bf16, [(0, 3, "v", np.nan), (0, 41, "k", -np.inf), (2, 70, "v", np.inf), (4, 1, "k", np.nan)],
+                members=[3, 1, 1], prefix=[48, 0, 0], tail=[1, 9, 40, 30, 21], seed=1, label="spoiled members")
+
+
+def run_faint(r, layer, bf16, keys=3000):
+    """One key far ahead of the others, which are as much together: each
+    probability is near 2^-12 of the largest and their sum is of its size.  The
+    tolerance of check_close counts 22 bits of each probability, not of the
+    largest one."""
+    rng = np.random.default_rng(11)
+    ps = 64
+    table = tables_for(rng, [keys], ps, -(-keys // ps) + 1)
+    pool = Pool(rng, 1, -(-keys // ps) + 1, r.hkv, ps, bf16, first_layer=layer, fill=0.0)
+    k, v = np.zeros((keys, r.hkv, D)), np.zeros((keys, r.hkv, D))
+    k[:, :, 0] = 1.0
+    k[0, :, 0] = 1.0 + 16 * np.log(keys) / 64.0      # q . k / 16 rises by log(keys)
+    v[...] = 1.0 + rng.standard_normal((1, 1, D)) / 4
+    v[0] = rng.standard_normal((r.hkv, D))
+    for p in range(keys):
+        pool.k[0, table[0, p // ps], :, p % ps] = pool.round(k[p])
+        pool.v[0, table[0, p // ps], :, p % ps] = pool.round(v[p])
+    q = np.zeros((1, r.hq, D), np.float32)
+    q[:, :, 0] = 64.0
+    want = packed_attention(pool, layer, r.span(layer), table, [keys], [0, 1], q)
+    r.pool(pool)
+    r.seqs(0, [keys], table)
+    r.prefill(layer, 0, [0, 1], q, lambda out: check_close(out, want, "faint keys, prefill"))
+    r.decode(layer, 0, None, q, lambda out: check_close(out, want, "faint keys, decode"))
+
+
+def run_serving(r, bf16, seed=0, rounds=4, ps=16):
+    """The five calls as a server makes them, checked call by call against the
+    oracles: prompts arrive, answers fork and grow, some end, the pool is
+    compacted, a chunk follows."""
+    rng = np.random.default_rng(seed)
+    layers, pages = 2, 40
+    pool = Pool(rng, layers, pages, r.hkv, ps, bf16, first_layer=4)       # layer 4 is local, 5 global
+    width = 12
+    lens, table = [0, 0, 0, 0], np.full((4, width), -1, np.int32)
+    r.pool(pool)
+    r.seqs(0, lens, table)
+    half = 2.0 ** -8 if bf16 else 0.0
+    qn, kn = to_bf16(rng.standard_normal(D) * 0.3), to_bf16(rng.standard_normal(D) * 0.3)
+
+    def step(parent, add, slot, groups=None):
+        """Fork, then per layer a write and the attention of the new tokens."""
+        nonlocal table, lens
+        parent, add = np.asarray(parent), np.asarray(add)
+        want_t, want_n, want_s, copies = fork(table, lens, parent, add, None, ps, pages)
+        assert want_s[1] == 0
+        r.seqs(slot, np.full(len(parent), -7), np.full(want_t.shape, -7, np.int32))
+        r.fork(1 - slot, parent, add, None, slot, lambda st: _same(st, want_s, "status"))
+        r.seqs_out(slot, want_t.shape, lambda n, t: (_same(n, want_n, "lengths"), _same(t, want_t, "tables")))
+        for src, dst, n in copies:
+            for a in (pool.k, pool.v):
+                a[:, dst, :, :n] = a[:, src, :, :n]
+        table, lens = want_t, [int(n) for n in want_n]
+        start = np.concatenate([[0], np.cumsum(add)])
+        n = int(start[-1])
+        for layer in (4, 5):
+            Q, K, V = (rng.standard_normal((n, h, D)).astype(np.float32) for h in (r.hq, r.hkv, r.hkv))
+            pos = np.concatenate([np.arange(lens[b] - add[b], lens[b]) for b in range(len(lens))])
+            wq, bq = (np.stack(x) for x in zip(*(norm_rope(Q[t], qn, r.rope(layer), p) for t, p in enumerate(pos))))
+            wk = np.stack([norm_rope(K[t], kn, r.rope(layer), p)[0] for t, p in enumerate(pos)])
+            for t, p in enumerate(pos):
+                b = int(np.searchsorted(start, t, "right")) - 1
+                page = table[b, p // ps]
+                pool.k[layer - 4, page, :, p % ps] = wk[t]
+                pool.v[layer - 4, page, :, p % ps] = V[t]
+            # what the attention reads is what was stored: off by the write's
+            # rounding from these values, which a score feels through 256 terms
+            # of either sign and an output directly
+            rel = REL + 20 * 2.0 ** -24 * 4 + half
+            want = packed_attention(pool, layer, r.span(layer), table, lens, start, wq.astype(np.float32))
+            r.write(layer, slot, start, Q, K, V, qn, kn, lambda out, w=wq, b=bq: _near(out, w, 20 * 2.0 ** -24 * b, "q"))
+            what = f"layer {layer} of {len(lens)} sequences"
+            wq32 = wq.astype(np.float32)
+            if np.all(add == 1):
+                r.decode(layer, slot, groups, wq32, lambda out, w=want, m=what: check_close(out, w, "decode " + m, rel))
+            else:
+                r.prefill(layer, slot, start, wq32, lambda out, w=want, m=what: check_close(out, w, "prefill " + m, rel))
+
+    def pack(slot):
+        nonlocal table
+        want_t, want_n, want_s, moves = compact(table, lens, None, ps, pages)
+        r.compact(slot, None, slot, lambda st: _same(st, want_s, "compact status"))
+        r.seqs_out(slot, want_t.shape, lambda n, t: (_same(n, want_n, "lengths"), _same(t, want_t, "tables")))
+        old_k, old_v = pool.k.copy(), pool.v.copy()
+        for s, d in moves:
+            pool.k[:, d], pool.v[:, d] = old_k[:, s], old_v[:, s]
+        table = want_t
+        return len(moves)
+
+    step([0, 1, 2], [37, 5, 50], 1)                          # three prompts
+    step([0, 0, 0, 1, 2, 2], [1] * 6, 0, ([0, 3, 4, 6], [37, 5, 50]))   # and their first answers, six of them
+    for i in range(rounds):
+        step(range(6), [1] * 6, 1, ([0, 3, 4, 6], [37, 0, 50]))
+        step(range(6), [1] * 6, 0, ([0, 3, 4, 6], [37, 0, 50]))
+    step([1, 3, 5, -1], [0, 3, 20, 0], 1)                    # half of them end, others go on, an empty one
+    assert pack(1) > 0
+    step([0, 1, 2, 3], [1, 1, 1, 33], 0)                     # is the next prompt
+    step([3, 0], [1, 1], 1)
+
+
+def _near(got, want, bound, what):
+    bad = np.abs(got - want) > bound
+    assert not bad.any(), f"{what}: {int(bad.sum())} off, worst {np.max(np.abs(got - want)):.2e}"

@@ -197,3 +197,178 @@ def test_refusals(run):
     ctx.paged_prefill_device(0, pages(), batch(0), None, None)      # nothing to do
     with G.Context(G.default_config(num_layers=1, max_context=16), 16, defer_rope=True) as bare:
         refused(bare.paged_write_device, 0, pages(num_layers=1, page_stride=4 * 16 * 256), batch(), A, A, A, None, None, A)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layer", [GLOBAL, LOCAL])
+def test_spoiled_keys(run, layer, bf16):
+    """An infinity or a NaN reaches the rows that see it and no others."""
+    P.run_spoiled_all(run(hq=4, hkv=2, window=32), layer, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_faint_keys(run, bf16):
+    P.run_faint(run(hq=4, hkv=2, max_context=8192), GLOBAL, bf16, keys=5000)
+
+
+@pytest.mark.parametrize("hq,hkv", HEADS)
+@pytest.mark.parametrize("seed", range(3))
+def test_decode_make_up(run, seed, hq, hkv):
+    """Runs of members, prefixes and tails of many lengths together."""
+    rng = np.random.default_rng(100 * seed + hq + hkv)
+    r = run(hq=hq, hkv=hkv, window=int(rng.integers(20, 600)), max_context=8192)
+    for i in range(3):
+        members = [int(m) for m in rng.integers(1, 40, int(rng.integers(1, 7)))]
+        n = sum(members)
+        prefix = [int(p) for p in rng.integers(0, 1500, len(members))]
+        tail = [int(t) for t in np.where(rng.random(n) < 0.8, rng.integers(0, 140, n), rng.integers(1, 1200, n))]
+        P.run_decode(r, [GLOBAL, LOCAL][int(rng.integers(2))], members, prefix, tail, [16, 64][int(rng.integers(2))], bool(rng.integers(2)),
+                     seed=seed * 10 + i, groups=bool(i), label=f"make-up {seed}.{i}")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_serving_loop(run, bf16):
+    P.run_serving(run(hq=8, hkv=4, window=24), bf16)
+
+
+class FarPages(P.GpuRunner):
+    """The pool's pages 2^28 elements apart, K and V of both layers beside each
+    other: byte and element offsets beyond 32 bits."""
+
+    def pool(self, p):
+        rows = p.hkv * p.ps * P.D
+        elem = 2 if p.bf16 else 4
+        self.p, stride = p, 1 << 28
+        buf = DeviceBuffer((p.pages - 1) * stride * elem + 2 * p.layers * rows * elem)
+        self.keep.append(buf)
+        self.pages = self.G.Pages(k=buf.ptr, v=buf.ptr + rows * elem, dtype=int(p.bf16), first_layer=p.first, num_layers=p.layers,
+                                  num_pages=p.pages, page_size=p.ps, page_stride=stride, layer_stride=2 * rows)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_far_pages(bf16):
+    r = FarPages(hq=4, hkv=2, window=24)
+    try:
+        P.run_serving(r, bf16, seed=3, rounds=1)
+    finally:
+        r.done()
+
+
+class Graphs:
+    """Capture and replay on a context's stream."""
+
+    def __init__(self, ctx):
+        self.hip, vp = DeviceBuffer.hip(), C.c_void_p
+        self.hip.hipStreamBeginCapture.argtypes = [vp, C.c_int]
+        self.hip.hipStreamEndCapture.argtypes = [vp, C.POINTER(vp)]
+        self.hip.hipGraphInstantiate.argtypes = [C.POINTER(vp), vp, vp, vp, C.c_size_t]
+        self.hip.hipGraphLaunch.argtypes = [vp, vp]
+        for f in ("hipGraphExecDestroy", "hipGraphDestroy"):
+            getattr(self.hip, f).argtypes = [vp]
+        self.ctx, self.stream, self.graph, self.exe = ctx, vp(ctx.stream()), vp(), vp()
+
+    def capture(self, calls):
+        assert self.hip.hipStreamBeginCapture(self.stream, 2) == 0        # hipStreamCaptureModeRelaxed
+        try:
+            calls()
+        finally:
+            assert self.hip.hipStreamEndCapture(self.stream, C.byref(self.graph)) == 0
+
+    def replay(self):
+        if not self.exe:
+            assert self.hip.hipGraphInstantiate(C.byref(self.exe), self.graph, None, None, 0) == 0
+        assert self.hip.hipGraphLaunch(self.exe, self.stream) == 0
+
+    def close(self):
+        if self.exe:
+            self.hip.hipGraphExecDestroy(self.exe)
+        if self.graph:
+            self.hip.hipGraphDestroy(self.graph)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_graph_replays(run, bf16):
+    """A step of a serving loop (every sequence grows by a token, is written,
+    decodes behind its shared prefix and sees its last rows again as a packed
+    prompt; then the pool is compacted) captured once and replayed, against the
+    same step called eagerly on a second pool.  Between replays the context
+    does other work in the same scratch memory.  The order of every sum is
+    fixed, so the results are the same bits."""
+    r = run(hq=8, hkv=4, window=40)
+    rng = np.random.default_rng(5)
+    ps, pages, lens, prefix = 16, 48, [100, 70, 66, 31], [64, 0]
+    first = [0, 3, 4]
+    B, width = len(lens), 12
+    table = P.tables_for(rng, lens, ps, pages, stride=width, shared=[(0, 3, 4)])
+    pool = P.Pool(rng, 1, pages, r.hkv, ps, bf16, first_layer=GLOBAL, fill=0.0)
+    pool.fill(rng, table, lens)
+    G, ctx = r.G, r.ctx
+    new = [r.buf(np.zeros((B, h, P.D), np.float32)) for h in (r.hq, r.hkv, r.hkv)]
+    qn, kn = (r.put(P.to_bf16(rng.standard_normal(P.D) * 0.3)) for _ in range(2))
+    groups = G.Prefixes(num_groups=2, group_start=r.put(np.asarray(first, np.int32)), prefix_len=r.put(np.asarray(prefix, np.int32)))
+    add = r.put(np.ones(B, np.int32))
+    rows = r.put(np.asarray([0, 2, 2, 4, 4], np.int32))        # two rows of the first, two of the third
+
+    class Server:
+        def __init__(self):
+            self.k, self.v = r.buf(pool.pack(pool.k)), r.buf(pool.pack(pool.v))
+            self.n, self.t = r.buf(np.asarray(lens, np.int32)), r.buf(table)
+            self.q, self.o, self.o2 = (r.buf(np.zeros((B, r.hq, P.D), np.float32)) for _ in range(3))
+            self.status = r.buf(np.zeros(4, np.int32))
+            self.pages = G.Pages(k=self.k.ptr, v=self.v.ptr, dtype=int(bf16), first_layer=GLOBAL, num_layers=1, num_pages=pages, page_size=ps,
+                                 page_stride=pool.page_stride, layer_stride=pool.layer_stride)
+            self.seqs = G.Seqs(num_seqs=B, kv_len=self.n.ptr, page_table=self.t.ptr, table_stride=width)
+
+        def step(self):
+            one = G.Batch(seqs=self.seqs, total_q=B, q_start=None)
+            ctx.pages_fork_device(self.pages, self.seqs, None, add, None, self.seqs, self.status.ptr)
+            ctx.paged_write_device(GLOBAL, self.pages, one, *(x.ptr for x in new), qn, kn, self.q.ptr)
+            ctx.paged_decode_device(GLOBAL, self.pages, one, groups, self.q.ptr, self.o.ptr)
+            ctx.paged_prefill_device(GLOBAL, self.pages, G.Batch(seqs=self.seqs, total_q=B, q_start=rows), self.q.ptr, self.o2.ptr)
+            ctx.pages_compact_device(self.pages, self.seqs, None, self.seqs, self.status.ptr + 8)
+
+        def state(self):
+            ctx.synchronize()
+            return [b.download(np.uint8, b.nbytes) for b in (self.n, self.t, self.status, self.q, self.o, self.o2, self.k, self.v)]
+
+    eager, graphed, other = Server(), Server(), Server()
+    other.step()                       # the scratch memory grows here
+    g = Graphs(ctx)
+    try:
+        g.capture(graphed.step)
+        for rep in range(5):
+            for b, h in zip(new, (r.hq, r.hkv, r.hkv)):
+                b.upload(rng.standard_normal((B, h, P.D)).astype(np.float32))
+            g.replay()
+            if rep < 3:
+                other.step()
+            eager.step()
+            for i, (a, b) in enumerate(zip(graphed.state(), eager.state())):
+                assert np.array_equal(a, b), f"replay {rep}, buffer {i}"
+    finally:
+        g.close()
+    assert list(eager.n.download(np.int32, B)) == [n + 5 for n in lens]
+
+
+def test_scratch_does_not_grow_under_capture(run):
+    """Refused with a message while the stream is captured, and fine after."""
+    r = run(hq=8, hkv=4, max_context=2048)
+    n = 200
+    q = np.zeros((n, r.hq, P.D), np.float32)
+    lens = [600] * n
+    table = np.zeros((n, 38), np.int32)
+    pool = P.Pool(np.random.default_rng(0), 1, 1, r.hkv, 16, False, first_layer=GLOBAL, fill=1.0)
+    r.pool(pool)
+    r.seqs(0, lens, table)
+    qb, out = r.buf(q), r.buf(q)
+    g = Graphs(r.ctx)
+
+    def refused():
+        with pytest.raises(r.G.G3AttnError) as e:
+            r.ctx.paged_decode_device(GLOBAL, r.pages, r.batch(0, n, None), None, qb.ptr, out.ptr)
+        assert e.value.rc == r.G.ERR_INVALID_ARG and "captured" in str(e.value)
+    try:
+        g.capture(refused)
+    finally:
+        g.close()
+    r.decode(GLOBAL, 0, None, q, lambda o: np.testing.assert_allclose(o, 1.0, rtol=1e-5))

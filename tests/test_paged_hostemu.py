@@ -185,3 +185,49 @@ def test_compact(built, tmp_path):
     P.run_compact(r, [0, 0], 16, 20, seed=4, label="empty")
     P.run_compact(r, [16] * 300, 16, 1500, seed=5, layers=1, label="large")
     r.done()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layer", [GLOBAL, LOCAL])
+def test_spoiled_keys(built, tmp_path, layer, bf16):
+    """An infinity or a NaN reaches the rows that see it and no others."""
+    r = P.EmuRunner(tmp_path, hq=4, hkv=2, window=32)
+    P.run_spoiled_all(r, layer, bf16)
+    r.done()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_faint_keys(built, tmp_path, bf16):
+    r = P.EmuRunner(tmp_path, hq=2, hkv=1, max_context=4096)
+    P.run_faint(r, GLOBAL, bf16, keys=1500)
+    r.done()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_decode_few_cus(built, tmp_path, seed):
+    """Batches of every make-up on 4 and 12 emulated CUs: chunks, second rounds,
+    packs of short sequences, odd chunk lengths."""
+    rng = np.random.default_rng(seed)
+    hq, hkv = [(2, 1), (4, 2), (4, 1)][seed % 3]
+    r = P.EmuRunner(tmp_path, env={"HOSTEMU_CUS": str([4, 12][seed % 2])}, hq=hq, hkv=hkv, window=int(rng.integers(20, 200)), max_context=2048)
+    for i in range(3):
+        members = [int(m) for m in rng.integers(1, 9, int(rng.integers(1, 6)))]
+        prefix = [int(p) for p in rng.integers(0, 300, len(members))]
+        tail = [int(t) for t in np.where(rng.random(sum(members)) < 0.7, rng.integers(0, 60, sum(members)), rng.integers(1, 400, sum(members)))]
+        P.run_decode(r, [GLOBAL, LOCAL][int(rng.integers(2))], members, prefix, tail, 16, bool(rng.integers(2)), seed=seed * 10 + i,
+                     groups=bool(i), label=f"few CUs {seed}.{i}")
+    r.done()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_serving_loop(built, tmp_path, bf16):
+    r = P.EmuRunner(tmp_path, hq=4, hkv=2, window=24)
+    P.run_serving(r, bf16, rounds=1)
+    r.done()
+
+
+def test_refusals(built, tmp_path):
+    """What the host can see is refused, before anything is touched."""
+    r = P.EmuRunner(tmp_path, hq=4, hkv=2)
+    r.lines.append("paged_refusals")
+    assert "attn_emu: refused" in r.done()
