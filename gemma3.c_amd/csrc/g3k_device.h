@@ -41,6 +41,7 @@
 
 #ifndef G3K_RECOMPUTE
 #define G3K_RECOMPUTE(x) asm volatile("" : "+v"(x))
+#define G3K_RECOMPUTE_S(x) asm volatile("" : "+s"(x))   // the same for a wave's value
 #endif
 
 // The XCD this wave runs on: the hardware register XCC_ID (gfx940 and

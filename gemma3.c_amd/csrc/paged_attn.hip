@@ -53,6 +53,7 @@ constexpr float M_NONE = -3.402823466e38f;  // running max before any key
 constexpr int E_NONE = -1000;               // running V exponent before any tile
 constexpr float LAZY = 8.0f;                // log2 headroom of the lazy max
 constexpr int P_EXP = 6;                    // P is scaled by 2^P_EXP: p <= 2^LAZY stays below 2^14
+constexpr int NOTES = 8;                    // of a tile: one per run and lane group; behind both tiles', unused ones
 constexpr int X_EXP = 14;                   // q, K, V: largest magnitude of a block below 2^X_EXP
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -91,14 +92,26 @@ __device__ __forceinline__ float wave_top(float v) {
     return col4_top(v);
 }
 
-// The power-of-two exponent of a block whose largest magnitude is m: m <
-// 2^exponent.  A block of zeros, or of values below 2^-100, counts as 2^-100;
-// one with an infinity or NaN as 2^127.
-__device__ __forceinline__ int block_exponent(float m) {
-    if (!(m < INFINITY)) return 127;
-    const int e = __builtin_amdgcn_frexp_expf(m);
-    return m == 0.f || e < -100 ? -100 : e;
+// The wave's largest of values >= 0, as bits: so ordered, NaN above all.
+__device__ __forceinline__ int wave_top_bits(float v) {
+    unsigned x = __float_as_uint(v);
+    const auto up = [&](unsigned y) { x = x > y ? x : y; };
+    up(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true));     // row_shr:1, 2, 4, 8
+    up(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true));
+    up(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true));
+    up(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true));
+    up(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));    // row_bcast:15 to rows 1 and 3
+    up(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));    // row_bcast:31 to rows 2 and 3
+    return __builtin_amdgcn_readlane((int)x, 63);
 }
+
+// The power-of-two exponent of a block whose largest magnitude has these bits:
+// it is below 2^exponent.  A block of zeros, or of values below 2^-100, counts
+// as 2^-100; one with an infinity or NaN as 2^129 (X_EXP - 129 is still the
+// exponent of a normal number).
+constexpr int NOT_FINITE = 0x7f800000;
+__device__ __forceinline__ int block_exponent(int bits) { return max((bits >> 23) - 126, -100); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // x s as hi + lo, two values at a time.
 __device__ __forceinline__ void split2(float a, float b, float s, half2v &hi, half2v &lo) {
@@ -166,17 +179,19 @@ __device__ __forceinline__ gbytes global_bytes(const void *p) { return (gbytes)p
 template <bool BF16, int NW>
 struct Finder {
     static constexpr int RUNS = 8 / NW, ROW = D * (BF16 ? 2 : 4);
-    // Of a wave's share of a tile: byte offsets of its runs' first rows from
-    // the head's first page; whether all rows are between kbeg and kend, and
-    // which runs have no page.
+    // A wave's share of a tile: byte offset of each run's first row from the
+    // head's first page, this lane's offsets of its rows from there, and which
+    // runs have no page.
     struct Place {
         long long off[RUNS];
-        int tile, bad;
+        unsigned row[4 * RUNS];
+        int bad, none;
     };
     const int *table;
     int shift, mask, last, pages, kbeg, kend;     // last: entry of the walk
     unsigned stride;                              // elements between pages
     int base, now, next;
+    gbytes zeros;
 
     __device__ __forceinline__ void begin(const g3k_paged_args &a, const Unit &u, int lane) {
         table = a.s.page_table + (long long)u.b * a.s.table_stride;
@@ -188,13 +203,14 @@ struct Finder {
         kbeg = u.kbeg;
         kend = u.kend;
         base = (kbeg >> shift) & ~63;
+        zeros = global_bytes(zero_row);
+        G3K_RECOMPUTE_S(zeros);
         now = table[clampi(base + lane, 0, last)];
         next = table[clampi(base + 64 + lane, 0, last)];
     }
     __device__ __forceinline__ Place place(int tile, int wave, int lane) {
         Place p;
-        p.tile = tile;
-        p.bad = 0;
+        p.bad = p.none = 0;
         const int j0 = tile * BK;
         if ((j0 >> shift) >= base + 64) {
             base += 64;
@@ -207,38 +223,29 @@ struct Finder {
             // (a run wholly outside the keys looks its nearest key's page up)
             const int e = clampi(j, kbeg & ~15, kend - 1) >> shift;
             const unsigned page = __builtin_amdgcn_readlane(now, e - base);
-            if (page >= (unsigned)pages) p.bad |= 1 << r;
+            // Keys outside [kbeg, kend) take the nearest row of their run
+            // inside, so nothing else is read; their scores are masked.  A page
+            // outside the pool is never followed, and neither is a run without
+            // a key: the rows are zeros.
+            const int from = max(kbeg - j, 0), to = min(kend - 1 - j, 15);
+            const bool bad = page >= (unsigned)pages, none = bad || from > to;
+            const int lo = none ? 0 : from, hi = none ? 0 : to;
+            if (bad) p.bad |= 1 << r;
+            if (none) p.none |= 1 << r;
             p.off[r] = (long long)(((unsigned long long)page * stride + (unsigned)((j & mask) * D)) * (BF16 ? 2 : 4));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                p.row[4 * r + i] = (unsigned)min(max(4 * (wave & 3) + i, lo), hi) * ROW + (unsigned)lane * (ROW / 64);
         }
         return p;
     }
-    // Fetches the rows.  Keys outside [kbeg, kend) take the nearest row of
-    // their run inside, so nothing else is read; their scores are masked.  A
-    // page outside the pool is never followed, and neither is a run without a
-    // key: the rows are zeros.
-    __device__ __forceinline__ void fetch(gbytes matrix, const Place &p, int wave, int lane, Raw<BF16, NW> &raw) const {
+    __device__ __forceinline__ void fetch(gbytes matrix, const Place &p, Raw<BF16, NW> &raw) const {
         using T = typename std::conditional<BF16, u32x2, f32x4>::type;
-        const int j0 = p.tile * BK;
-        if (j0 >= kbeg && j0 + BK <= kend && !p.bad) {
-#pragma unroll
-            for (int r = 0; r < RUNS; r++) {
-                const gbytes row = matrix + p.off[r] + 4 * (wave & 3) * ROW;
-#pragma unroll
-                for (int i = 0; i < 4; i++) raw.x[4 * r + i] = load_global<T>(row + i * ROW + lane * (int)sizeof(T));
-            }
-            return;
-        }
 #pragma unroll
         for (int r = 0; r < RUNS; r++) {
-            const int j = j0 + 16 * (NW == 4 ? r : wave >> 2);
-            const int lo = max(j, kbeg), hi = min(j + 16, kend) - 1;      // the run's keys
-            const bool none = lo > hi || ((p.bad >> r) & 1);
+            const gbytes rows = (p.none >> r) & 1 ? zeros : matrix + p.off[r];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int k = clampi(j + 4 * (wave & 3) + i, lo, hi) - j;
-                const gbytes row = none ? global_bytes(zero_row) : matrix + p.off[r] + k * ROW;
-                raw.x[4 * r + i] = load_global<T>(row + lane * (int)sizeof(T));
-            }
+            for (int i = 0; i < 4; i++) raw.x[4 * r + i] = load_global<T>(rows + p.row[4 * r + i]);
         }
     }
 };
@@ -256,14 +263,14 @@ __device__ __forceinline__ float rows_max(const Raw<BF16, NW> &raw) {
     return m;
 }
 
-// The largest finite magnitude of this wave's rows in flight, where some hold
+// The largest finite magnitude (its bits) of this wave's rows in flight, where some hold
 // an infinity or a NaN (seldom any): those rows, one bit each in `spoiled`, are
 // left out of the exponent, which is their neighbours' too.  K's become NaN,
 // and so their scores, which are masked for the rows that do not see them.
 // V's become zeros, since a value that is not finite times p = 0 is NaN in
 // every row of the product; a row that sees the key is made NaN instead.
 template <bool KEYS, bool BF16, int NW>
-__device__ __forceinline__ float settle(Raw<BF16, NW> &raw, int &spoiled) {
+__device__ __forceinline__ int settle(Raw<BF16, NW> &raw, int &spoiled) {
     spoiled = 0;
     float most = 0.f;
 #pragma unroll
@@ -277,7 +284,7 @@ __device__ __forceinline__ float settle(Raw<BF16, NW> &raw, int &spoiled) {
             most = top(most, y);
         }
     }
-    return wave_top(most);
+    return wave_top_bits(most);
 }
 
 // K's rows (exponent e over the wave) as operands: lane holds dims 4 lane.. = half (lane & 1) of operand
@@ -286,13 +293,13 @@ __device__ __forceinline__ float settle(Raw<BF16, NW> &raw, int &spoiled) {
 template <bool BF16, int NW>
 __device__ __forceinline__ void store_k(const Raw<BF16, NW> &raw, int e, int bad, char *buf, f32x2 *factors, int wave, int lane) {
     using L = Lds<BF16>;
-    const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
+    const float sc = pow2(X_EXP - e);
     char *kd = buf + (lane >> 3) * (L::PL * 1024) + ((lane >> 1) & 3) * 256 + (lane & 1) * 8;
     const int f = (lane >> 1) & 15;
 #pragma unroll
     for (int r = 0; r < Raw<BF16, NW>::RUNS; r++) {
         const int c = NW == 4 ? r : wave >> 2;
-        if (lane == 0) factors[4 * c + (wave & 3)] = (f32x2){__builtin_amdgcn_ldexpf(1.0f, e - X_EXP), (bad >> r) & 1 ? -INFINITY : 0.f};
+        factors[lane ? 2 * NOTES + lane : 4 * c + (wave & 3)] = (f32x2){pow2(e - X_EXP), (bad >> r) & 1 ? -INFINITY : 0.f};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const f32x4 x = raw.get(4 * r + i);
@@ -325,9 +332,11 @@ __device__ __forceinline__ void store_v(const Raw<BF16, NW> &raw, int e, int spo
     using L = Lds<BF16>;
     constexpr int N = 4 * Raw<BF16, NW>::RUNS;
     typedef _Float16 Keys __attribute__((ext_vector_type(N)));
-    const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
+    const float sc = pow2(X_EXP - e);
     const int c = NW == 4 ? 0 : wave >> 2;
-    if (lane < 8 / NW) exps[4 * (NW == 4 ? lane : c) + (wave & 3)] = e + ((spoiled >> 4 * lane & 15) << 12);
+    // (with 4 waves lane 1 has the second run's)
+    const int run = NW == 4 ? lane & 1 : 0;
+    exps[lane < 8 / NW ? 4 * (c + run) + (wave & 3) : 2 * NOTES + lane] = e + ((spoiled >> 4 * run & 15) << 12);
     char *vd = buf + (lane >> 4) * (4 * L::PL * 1024) + (wave & 3) * 256 + (lane & 15) * 16 + c * 8;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -361,37 +370,40 @@ struct Rows {
     int ev;                           // O^T's exponent: o = true o * 2^(X_EXP + P_EXP - ev), unnormalised
 };
 
-__device__ __forceinline__ void load_query(const float *q, bool live, float qscale, int lane, Rows &s) {
-    float x[8][8];
-    float m = 0.f;
+// A row's query: this lane group's 8 of every 32 dims, and their split planes.
+struct Query {
+    f32x4 x[8][2];
+    __device__ __forceinline__ void load(const float *q, bool live, int lane) {
 #pragma unroll
-    for (int kk = 0; kk < 8; kk++) {
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        const float *p = q + 32 * kk + 8 * (lane >> 4);
-        const f32x4 a = live ? *reinterpret_cast<const f32x4 *>(p) : z;
-        const f32x4 b = live ? *reinterpret_cast<const f32x4 *>(p + 4) : z;
+        for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[kk][i] = a[i];
-            x[kk][4 + i] = b[i];
-            m = top(top(m, fabsf(a[i])), fabsf(b[i]));
-        }
+            for (int i = 0; i < 2; i++) {
+                const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                x[kk][i] = live ? *reinterpret_cast<const f32x4 *>(q + 32 * kk + 8 * (lane >> 4) + 4 * i) : z;
+            }
     }
-    const int e = block_exponent(col4_top(m));
-    const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
-    s.factor = __builtin_amdgcn_ldexpf(qscale, e - X_EXP);
+    __device__ __forceinline__ void split(float qscale, Rows &s) const {
+        float m = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < 8; kk++)
+        for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            half2v h, l;
-            split2(x[kk][i], x[kk][i + 1], sc, h, l);
-            s.qh[kk][i] = h.x;
-            s.qh[kk][i + 1] = h.y;
-            s.ql[kk][i] = l.x;
-            s.ql[kk][i + 1] = l.y;
-        }
-}
+            for (int i = 0; i < 8; i++) m = top(m, fabsf(x[kk][i >> 2][i & 3]));
+        const int e = block_exponent(__float_as_int(col4_top(m)));
+        const float sc = pow2(X_EXP - e);
+        s.factor = __builtin_amdgcn_ldexpf(qscale, e - X_EXP);
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v h, l;
+                split2(x[kk][i >> 2][i & 3], x[kk][i >> 2][(i & 3) + 1], sc, h, l);
+                s.qh[kk][i] = h.x;
+                s.qh[kk][i + 1] = h.y;
+                s.ql[kk][i] = l.x;
+                s.ql[kk][i + 1] = l.y;
+            }
+    }
+};
 
 // S^T of a tile.
 template <bool BF16>
@@ -467,7 +479,7 @@ __device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, in
         s.l *= keep;
 #pragma unroll
         for (int d = 0; d < 16; d++) s.o[d] *= keep;
-        if (__builtin_amdgcn_ballot_w64(also)) other();
+        if (also) other();
     }
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
@@ -558,12 +570,12 @@ __device__ __forceinline__ void tile_values(const char *buf, int lane, half8 ph,
 // rows of later tiles split and stored (and the next ones fetched).  With 8
 // waves, waves w and w + 4 share a SIMD; the second four run one phase later,
 // so that one is in M while the other is in V, and store one tile further
-// ahead (`lead`).  Tile i + 2 of K goes where tile i was, i + 1 of V where i - 1
+// ahead (`lead`).  q: this lane's row's query, if it is live.  Tile i + 2 of K goes where tile i was, i + 1 of V where i - 1
 // was, both at least a phase after their last read and before their first;
 // what V(i) needs of the factors is read in M(i), before others write them.
 template <bool BF16, int NW>
 __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Unit &u, char *lds, f32x2 *factors, int *exps, int wave,
-                                     int lane, Rows &s) {
+                                     int lane, const float *q, bool live, Rows &s) {
     using L = Lds<BF16>;
     const int t0 = u.kbeg / BK, n = u.kend > u.kbeg ? (u.kend + BK - 1) / BK - t0 : 0;
     if (n <= 0) return;
@@ -571,24 +583,29 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
     const long long head_off = ((long long)head << a.s.page_shift) * D * (BF16 ? 2 : 4);
     const gbytes kb = global_bytes(a.k) + head_off, vb = global_bytes(a.v) + head_off;
     Finder<BF16, NW> find;
+    // the pages, the query and the first rows are asked for before any is used
+    // (9 short prompts 22.2 us; 22.9 with the query settled first)
     find.begin(a, u, lane);
+    Query query;
+    query.load(q, live, lane);
     Raw<BF16, NW> rk, rv;
     int ik = 0, iv = 0;       // tiles in flight; past the end, the last one again
     auto pk = find.place(t0, wave, lane), pv = pk;
-    find.fetch(kb, pk, wave, lane, rk);
-    find.fetch(vb, pv, wave, lane, rv);
+    find.fetch(kb, pk, rk);
+    find.fetch(vb, pv, rv);
+    query.split(a.qscale, s);
     // K's next tile has been looked up when V's is fetched
     const auto next_k = [&](int e) {
         store_k<BF16, NW>(rk, e, pk.bad, kbuf + (ik & 1) * L::K_BYTES, factors + 8 * (ik & 1), wave, lane);
         ik++;
         pv = pk;
         pk = find.place(t0 + min(ik, n - 1), wave, lane);
-        find.fetch(kb, pk, wave, lane, rk);
+        find.fetch(kb, pk, rk);
     };
     const auto next_v = [&](int e, int spoiled) {
         store_v<BF16, NW>(rv, e, spoiled, vbuf + (iv & 1) * L::V_BYTES, exps + 8 * (iv & 1), wave, lane);
         iv++;
-        find.fetch(vb, pv, wave, lane, rv);
+        find.fetch(vb, pv, rv);
     };
     const int lead = NW == 8 ? wave >> 2 : 0;
     int spoiled;
@@ -622,9 +639,9 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         if (NW == 8) G3K_WAIT_BARRIER(63);
         // V(i - 1)
         // (three chains of cross-lane steps side by side)
-        float mk = wave_top(rows_max<BF16, NW>(rk)), mv = wave_top(rows_max<BF16, NW>(rv));
+        int mk = wave_top_bits(rows_max<BF16, NW>(rk)), mv = wave_top_bits(rows_max<BF16, NW>(rv));
         spoiled = 0;
-        tile_softmax(fac, t, lane, s, p, !(top(mk, mv) < INFINITY), [&]() {
+        tile_softmax(fac, t, lane, s, p, max(mk, mv) >= NOT_FINITE, [&]() {
             mk = settle<true>(rk, spoiled);
             mv = settle<false>(rv, spoiled);
         });
@@ -688,12 +705,15 @@ struct Prompt {
         const int whole = (max(pos + n, 0) + BK - 1) / BK;
         return all ? whole : min(whole, (a.window + T) / BK + 2);
     }
-    // the first block with more than p chunks of c tiles (or an earlier one,
-    // behind a window): a block's keys end with it
-    __device__ __forceinline__ int first_with(int p, int c, int T) const {
-        const int x = p * c * BK - pos;
-        return p == 0 || !all || x < 0 ? 0 : min(x / T, blocks);
+    // the first block with x tiles or more (`blocks`: none); a block's keys end
+    // with it
+    __device__ __forceinline__ int first_of(int x, int T) const {
+        const int y = (x - 1) * BK - pos;
+        return x <= 0 || y < 0 ? 0 : y >= n ? blocks : y >> __builtin_ctz(T);      // (T is a power of two)
     }
+    // the first with more than p chunks of c tiles (or an earlier one, behind a
+    // window)
+    __device__ __forceinline__ int first_with(int p, int c, int T) const { return p == 0 || !all ? 0 : first_of(p * c + 1, T); }
     __device__ __forceinline__ int chunks(const g3k_paged_args &a, int c, int T) const {
         const int t = most_tiles(a, T);
         return t > 0 ? (t + c - 1) / c : 1;
@@ -713,7 +733,7 @@ __device__ __forceinline__ Prompt prompt_of(const g3k_paged_args &a, int b, int 
     seq_rows(a.s, b, p.first, p.n);
     const int len = seq_len(a.s, b);
     p.pos = len - p.n;
-    p.blocks = (p.n + T - 1) / T;
+    p.blocks = (p.n + T - 1) >> __builtin_ctz(T);
     p.all = a.window >= len;
     return p;
 }
@@ -765,9 +785,85 @@ __device__ __forceinline__ Prompt uniform(const Prompt &p, int lane) {
     return r;
 }
 
-// Item `item` of the batch: chunk by chunk of each sequence, its last block
-// (the one with the most keys) first.  False past the last item.
-__device__ bool find_item(const g3k_paged_args &a, int item, int c, int T, int lane, Unit &u, int &chunk) {
+// Items of a batch of up to 64 sequences run longest first, in classes:
+// whole chunks, then the last ones of blocks from 3/4, 1/2, 1/4, 1/8 of one and
+// from nothing, so that the CUs end together (5 bf16 chunks behind cached
+// keys 282 us, sequence by sequence 307).  Class 0 holds chunk p of blocks with
+// p + 1 whole ones, class k chunk p of blocks with p c + [lo, hi) tiles.
+constexpr int CLASSES = 6;
+struct Classes {
+    int c, T;
+    // least tiles, beyond p chunks, of classes i and before
+    __device__ __forceinline__ int least(int i, int p) const { return i == 0 ? c : i < 5 ? max(c * (0x1246 >> 4 * (i - 1) & 15) >> 3, 1) : p == 0 ? 0 : 1; }
+    // class k's blocks of which chunk p is one: [from, to)
+    __device__ __forceinline__ void blocks(const Prompt &s, int k, int p, int &from, int &to) const {
+        from = s.first_of(p * c + least(k, p), T);
+        to = k ? s.first_of(p * c + least(k - 1, p), T) : s.blocks;
+    }
+    __device__ __forceinline__ void count(const g3k_paged_args &a, const Prompt &s, int (&n)[CLASSES]) const {
+#pragma unroll
+        for (int k = 0; k < CLASSES; k++) n[k] = 0;
+        if (s.blocks == 0) return;
+        if (!s.all) {
+            n[0] = s.blocks * s.chunks(a, c, T);
+            return;
+        }
+        const int most = s.most_tiles(a, T);
+        for (int p = 0; p * c <= most; p++) {
+            int to = s.blocks;
+#pragma unroll
+            for (int k = 0; k < CLASSES; k++) {
+                const int from = s.first_of(p * c + least(k, p), T);
+                n[k] += to - from;
+                to = from;
+            }
+        }
+    }
+};
+
+// What workgroup `item` of the batch does: a block's rows and a chunk of its
+// keys, and where the chunk's part goes: slots count chunk by chunk of each
+// sequence, its last block first.  False past the last item.
+__device__ bool find_item(const g3k_paged_args &a, int item, int c, int T, int lane, Unit &u, int &chunk, int &slot) {
+    if (a.budget > 0 && a.s.num_seqs <= 64) {
+        const Prompt mine = prompt_of(a, lane, T);
+        const int slots = mine.blocks > 0 ? mine.items(a, c, T) : 0;
+        const Classes classes = {c, T};
+        int counts[CLASSES], before = 0;
+        classes.count(a, mine, counts);
+#pragma unroll
+        for (int cls = 0; cls < CLASSES; cls++) {
+            const int n = counts[cls], upto = wave_scan_int(n);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(item - before < upto);
+            if (!past) {
+                before += __builtin_amdgcn_readlane(upto, 63);
+                continue;
+            }
+            const int at = __builtin_ctzll(past);
+            const Prompt p = uniform(mine, at);
+            int k = item - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at)), rb;
+            if (p.all) {
+                for (chunk = 0;; chunk++) {
+                    int from, to;
+                    classes.blocks(p, cls, chunk, from, to);
+                    if (k < to - from) {
+                        rb = to - 1 - k;
+                        break;
+                    }
+                    k -= to - from;
+                }
+            } else {
+                chunk = k / p.blocks;
+                rb = p.blocks - 1 - k % p.blocks;
+            }
+            slot = __builtin_amdgcn_readlane(wave_scan_int(slots), at) - __builtin_amdgcn_readlane(slots, at) + p.blocks - 1 - rb;
+            for (int q = 0; q < chunk; q++) slot += p.blocks - p.first_with(q, c, T);
+            set_block(a, at, p, rb, T, u);
+            return slot < a.items;      // (not so where rows of sequences overlap)
+        }
+        return false;
+    }
+    slot = item;
     int before = 0;
     for (int base = 0; base < a.s.num_seqs; base += 64) {
         const Prompt mine = prompt_of(a, base + lane, T);
@@ -794,16 +890,16 @@ __device__ bool find_item(const g3k_paged_args &a, int item, int c, int T, int l
 template <bool BF16, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void paged_prefill_kernel(g3k_paged_args a) {
     __shared__ __align__(16) char lds[Lds<BF16>::BYTES];
-    __shared__ f32x2 factors[16];
-    __shared__ int exps[16];
+    __shared__ f32x2 factors[3 * NOTES + 64];
+    __shared__ int exps[3 * NOTES + 64];
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.n_kv_heads, item = blockIdx.x / a.n_kv_heads;
     constexpr int ROWS = 16 * NW;
     Unit u;
-    int chunk;
+    int chunk, part;
     const int T = ROWS / a.group, c = __builtin_amdgcn_readfirstlane(prompt_chunk(a, T, lane));
-    if (!find_item(a, item, c, T, lane, u, chunk)) return;
+    if (!find_item(a, item, c, T, lane, u, chunk, part)) return;
     const int parts = block_chunks(u, c);
     if (chunk >= parts) return;
     const int kbeg = max(u.kbeg, (u.kbeg / BK + chunk * c) * BK), kend = min((long long)u.kend, (u.kbeg / BK + (chunk + 1LL) * c) * BK);
@@ -816,19 +912,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_prefill_kernel(g3k_page
         const int hi = u.pos + tok + 1;
         s.hi = live ? min(hi, kend) : INT_MAX;
         s.lo = live ? max(hi - a.window, kbeg) : 0;
-        load_query(a.q + ((long long)(u.run + tok) * a.n_kv_heads * a.group + h) * D, live, a.qscale, lane, s);
+        begin_rows(s);
+        u.kbeg = kbeg;
+        u.kend = kend;
+        walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane,
+                       a.q + ((long long)(u.run + tok) * a.n_kv_heads * a.group + h) * D, live, s);
     }
-    begin_rows(s);
-    u.kbeg = kbeg;
-    u.kend = kend;
-    walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, s);
     G3K_RECOMPUTE(lane);      // no output address is kept through the walk
     {
         const int row = wave * 16 + (lane & 15);
         float *out = nullptr, *ml = nullptr;
         if (row < u.count) {
             if (parts > 1) {
-                const long long slot = ((long long)item * a.n_kv_heads + head) * ROWS + row;
+                const long long slot = ((long long)part * a.n_kv_heads + head) * ROWS + row;
                 out = a.part_o + slot * D;
                 ml = a.part_ml + slot * 2;
             } else {
@@ -1187,7 +1283,7 @@ __device__ __forceinline__ float bf16_of(const u32x4 &x, int i) {
 __device__ __forceinline__ float f32_of(const u32x4 &x, int i) { return __uint_as_float(x[i]); }
 
 template <bool BF16>
-__device__ __forceinline__ float step_max(const u32x4 (&x)[BF16 ? 8 : 16]) {
+__device__ __forceinline__ int step_max(const u32x4 (&x)[BF16 ? 8 : 16]) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < (BF16 ? 8 : 16); i++)
@@ -1195,7 +1291,7 @@ __device__ __forceinline__ float step_max(const u32x4 (&x)[BF16 ? 8 : 16]) {
         for (int e = 0; e < (BF16 ? 8 : 4); e += 2)
             m = BF16 ? top(top(m, fabsf(bf16_of(x[i], e))), fabsf(bf16_of(x[i], e + 1)))
                      : top(top(m, fabsf(f32_of(x[i], e))), fabsf(f32_of(x[i], e + 1)));
-    return wave_top(m);
+    return wave_top_bits(m);
 }
 
 // The dim of element i of dim step kk's operand lane of group g: K's loads are
@@ -1277,7 +1373,7 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
         for (int kk = 0; kk < 8; kk++)
 #pragma unroll
             for (int i = 0; i < 8; i++) m = top(m, fabsf(xq[kk][i >> 2][i & 3]));
-        const int e = block_exponent(col4_top(m));
+        const int e = block_exponent(__float_as_int(col4_top(m)));
         const float sc = __builtin_amdgcn_ldexpf(1.0f, X_EXP - e);
         qfac = __builtin_amdgcn_ldexpf(a.qscale, e - X_EXP);
 #pragma unroll
@@ -1302,7 +1398,7 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
         const int first = begin(n), fin = end(n);
         const bool gone = w.rs == 0;
         G3K_RECOMPUTE(lane);
-        const float mk = step_max<BF16>(x.k);
+        const int mk = step_max<BF16>(x.k);
         const int ek = block_exponent(mk);
         const float sk = __builtin_amdgcn_ldexpf(1.0f, X_EXP - ek);
         f32x4 sc = {0.f, 0.f, 0.f, 0.f}, sx = sc, sy = sc;
@@ -1345,8 +1441,8 @@ __device__ __forceinline__ void walk_tail(const g3k_paged_args &a, int head, con
             t = top(t, sc[r]);
         }
         t = col4_top(t);
-        const float mv = step_max<BF16>(x.v);
-        if (!(mk < INFINITY) || !(mv < INFINITY)) s.l = NAN;     // every head sees the step's rows
+        const int mv = step_max<BF16>(x.v);
+        if (max(mk, mv) >= NOT_FINITE) s.l = NAN;     // every head sees the step's rows
         const int ev = block_exponent(mv);
         const bool up = t > s.m + LAZY;
         if (__builtin_amdgcn_ballot_w64(up) || ev > s.ev) {
@@ -1470,8 +1566,8 @@ template <bool BF16>
 __global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_decode_kernel(g3k_paged_args a) {
     constexpr int NW = DECODE_WAVES;
     __shared__ __align__(16) char lds[Lds<BF16>::BYTES];
-    __shared__ f32x2 factors[16];
-    __shared__ int exps[16];
+    __shared__ f32x2 factors[3 * NOTES + 64];
+    __shared__ int exps[3 * NOTES + 64];
     constexpr int ROWS = 16 * NW;
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1520,10 +1616,9 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_dec
         const int len = live ? seq_len(a.s, seq) : 0;
         s.hi = live ? min(len, u.kend) : INT_MAX;
         s.lo = live ? max(len - a.window, u.kbeg) : 0;
-        load_query(a.q + ((long long)seq * a.n_kv_heads * a.group + h) * D, live, a.qscale, lane, s);
+        begin_rows(s);
+        walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, a.q + ((long long)seq * a.n_kv_heads * a.group + h) * D, live, s);
     }
-    begin_rows(s);
-    walk<BF16, NW>(a, head, u, lds, factors, exps, wave, lane, s);
     G3K_RECOMPUTE(lane);      // no output address is kept through the walk
     const int row = wave * 16 + (lane & 15);
     const long long slot = slot0 + row;

@@ -100,6 +100,7 @@ hipError_t hipOccupancyMaxActiveBlocksPerMultiprocessor(int *n, K, int, size_t) 
 #define G3K_WAIT_VMEM() hostemu::complete_fetches(0)
 #define G3K_WAIT_BARRIER(n) (hostemu::complete_fetches(n), hostemu::machine()->block.wait())
 #define G3K_RECOMPUTE(x) ((void)(x))
+#define G3K_RECOMPUTE_S(x) ((void)(x))
 #define G3K_GLOBAL
 #define G3K_ORDER_FENCE() ((void)hostemu::machine()->current->fence++)
 // The emulated machine deals workgroup i to XCD i mod 8, as the MI355X
