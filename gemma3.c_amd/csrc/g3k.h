@@ -403,9 +403,11 @@ int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
  * Decode: group i's members [group_start[i], group_start[i + 1]) share their
  * first prefix_len[i] positions, read once per G3K_PAGED_DECODE_ROWS rows
  * through the first member's table.
- * The keys are cut into about `budget` chunks per KV head, at most `items`,
- * of at least min_tiles 32-key tiles; with `pack`, short sequences are one
- * wave's work.  Parts [items][n_kv_heads][part_rows]
+ * The keys are cut into about `budget` chunks per KV head (or 2 for each run
+ * of keys), at most `items` = max(budget, 2 runs) + runs, of at least min_tiles
+ * 32-key tiles; runs: sequences, and for groups one each and one per
+ * G3K_PAGED_DECODE_ROWS rows.  With `pack`, short sequences are one wave's
+ * work.  Parts [items][n_kv_heads][part_rows]
  * rows, found through the directories dir_prefix and dir_tail [num_seqs][4]. */
 typedef struct {
     g3k_paged_seqs s;

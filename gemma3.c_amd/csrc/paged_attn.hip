@@ -1114,12 +1114,15 @@ __device__ __forceinline__ SeqLane seq_lane(const g3k_paged_args &a, int b) {
     return s;
 }
 
-// The units' keys are cut into chunks of about equal work, as many as make at
-// most a.budget items per KV head, whatever the lengths: every wave adds the
-// lengths up for itself, then finds its item.  One item more than there are
-// CUs costs a second round of workgroups (8 unrelated sequences, 313 tiles: 36
-// us with 67 items a head, 21 with 64), so where the lengths are all in
-// registers the chunks are lengthened until the count fits.
+// The units' keys are cut into chunks of about equal work, as many as make
+// a.budget items per KV head (one per CU), whatever the lengths: every wave
+// adds the lengths up for itself, then finds its item.  One item more than
+// there are CUs costs a second round of workgroups (8 unrelated sequences, 313
+// tiles: 36 us with 67 items a head, 21 with 64), so where the lengths are all
+// in registers the chunks are lengthened until the count fits.  Where units
+// are more than half the CUs, twice as many items as units, or the long ones
+// would hardly be cut (48 sequences in 3 groups, bf16: 77 us; 1.5 times as many
+// 79, as many 148, 2.5 times 91).
 struct DecodePlan {
     GroupLane g0;
     SeqLane s0;
@@ -1149,7 +1152,7 @@ struct DecodePlan {
         alone = a.pack ? wave_sum_int(alone) : 0;
         const int packs = (alone + waves - 1) / waves;
         units = a.s.num_seqs - alone + (a.n_groups ? wave_sum_int(units) : 0);
-        const int budget = max(a.budget - packs, 1);
+        const int budget = max(a.budget, (units + packs) * 2) - packs;
         const int room = all ? budget : max(budget - units, budget / 2);
         const float c = total * 1.0001f / (float)max(room, 1) + 1.0f;
         per = c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
@@ -1177,7 +1180,31 @@ __device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int
         u.kbeg = max(kbeg, t0 * BK);
         u.kend = min(kend, (t0 + each) * BK);
     };
-    int before = 0;
+    const int packs = (plan.alone + waves - 1) / waves;
+    if (item < packs) {      // first: one wave on its own is long at it
+        r.any = r.alone = true;
+        const int k = item * waves + wave;
+        u.b = u.run = u.pos = u.kbeg = u.kend = 0;
+        u.count = a.group;
+        int before = 0;
+        for (int base = 0; base < a.s.num_seqs; base += 64) {
+            const SeqLane s = base ? seq_lane(a, base + lane) : plan.s0;
+            const int upto = wave_scan_int(s.alone > 0);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(k - before < upto);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                r.chunks = 1;
+                r.shares = at(s.shares, l) > 0;
+                u.b = u.run = base + l;
+                u.kbeg = at(s.kbeg, l);
+                u.kend = at(s.len, l);
+                return r;
+            }
+            before += at(upto, 63);
+        }
+        return r;
+    }
+    int before = packs;
     for (int base = 0; base < a.n_groups; base += 64) {
         const GroupLane g = base ? group_lane(a, base + lane, rows) : plan.g0;
         const int c = plan.prefix_chunks(g.tiles);
@@ -1215,27 +1242,6 @@ __device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int
             u.count = a.group;
             u.pos = 0;
             keys(at(s.kbeg, l), at(s.len, l), at(s.tiles, l));
-            return r;
-        }
-        before += at(upto, 63);
-    }
-    if ((item - before) * waves >= plan.alone) return r;
-    r.any = r.alone = true;
-    const int k = (item - before) * waves + wave;
-    u.b = u.run = u.pos = u.kbeg = u.kend = 0;
-    u.count = a.group;
-    before = 0;
-    for (int base = 0; base < a.s.num_seqs; base += 64) {
-        const SeqLane s = base ? seq_lane(a, base + lane) : plan.s0;
-        const int upto = wave_scan_int(s.alone > 0);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(k - before < upto);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            r.chunks = 1;
-            r.shares = at(s.shares, l) > 0;
-            u.b = u.run = base + l;
-            u.kbeg = at(s.kbeg, l);
-            u.kend = at(s.len, l);
             return r;
         }
         before += at(upto, 63);

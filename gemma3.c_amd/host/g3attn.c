@@ -2536,16 +2536,14 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
         a.prefix_len = prefixes->prefix_len;
     }
     const int rows = G3K_PAGED_DECODE_ROWS;
-    /* Per KV head one chunk a CU, or as many as there are runs of keys (4 KV
-     * heads, 64 sequences behind 8192 keys: 55 us; 8 heads, 48 sequences in 3
-     * groups, bf16: 83; half as many as runs 53, 151; twice as many 81, 91);
-     * the last chunk of a run is a part one.  With more runs than CUs short sequences
-     * are one wave's work (same two: 106, 151 us if not). */
+    /* Per KV head one chunk a CU, or two for each run of keys; the last chunk
+     * of a run is a part one.  With more runs than CUs short sequences are one
+     * wave's work (4 KV heads, 64 sequences behind 8192 keys; 8 heads, 48 in 3
+     * groups, bf16: 55, 83 us, otherwise 106, 151). */
     const int units = B + (a.n_groups ? a.n_groups + B * c->group / rows : 0);
     a.budget = (c->n_cu + Hkv - 1) / Hkv;
-    if (a.budget < units) a.budget = units;
     a.pack = (long long)units * Hkv > c->n_cu;
-    a.items = a.budget + units;
+    a.items = (a.budget > 2 * units ? a.budget : 2 * units) + units;
     a.min_tiles = 2;
     a.part_rows = a.n_groups ? rows : c->group;
     const size_t n = (size_t)a.items * Hkv * a.part_rows, ob = align256(n * D * sizeof(float)), mb = align256(n * 2 * sizeof(float));
