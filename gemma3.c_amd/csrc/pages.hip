@@ -21,7 +21,7 @@
 //
 // pages_compact: the pages in use move to the lowest numbers.
 //
-// Both are integers over tables (latency: four launches), then copies of
+// Both are integers over tables (latency: two to four launches), then copies of
 // rows of every layer's K and V (bytes).
 #include <hip/hip_runtime.h>
 #include <limits.h>
@@ -153,26 +153,31 @@ __global__ __launch_bounds__(256) void paged_write_kernel(g3k_paged_write_args a
 
 // ---- counting -------------------------------------------------------------------
 
+// Per page: how many sequences hold it, and of children that are going to write
+// it how many there are and the first one.
+struct Counts {
+    int *ref, *writers, *first;
+};
+
 // Counts start from the caller's own holds.
-__global__ __launch_bounds__(256) void pages_clear_kernel(g3k_pages_args a) {
-    const int p = blockIdx.x * 256 + threadIdx.x;
-    if (p >= a.num_pages) return;
-    a.ref[p] = a.held && a.held[p] ? 1 : 0;
-    if (a.writers) {
-        a.writers[p] = 0;
-        a.first[p] = INT_MAX;
+__device__ __forceinline__ void clear_page(const g3k_pages_args &a, const Counts &n, int p) {
+    n.ref[p] = a.held && a.held[p] ? 1 : 0;
+    if (n.writers) {
+        n.writers[p] = 0;
+        n.first[p] = INT_MAX;
     }
     if (a.map) a.map[p] = p;
+}
+__global__ __launch_bounds__(256) void pages_clear_kernel(g3k_pages_args a) {
+    const int p = blockIdx.x * 256 + threadIdx.x;
+    if (p < a.num_pages) clear_page(a, {a.ref, a.writers, a.first}, p);
 }
 
 __device__ __forceinline__ int pages_of(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
 
-// One wave per child: what it keeps of its parent, and its claim on the last
-// page if it is going to write there.
-__global__ __launch_bounds__(256) void fork_count_kernel(g3k_pages_args a) {
-    const int lane = threadIdx.x & 63;
-    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= a.n_out) return;
+// One wave: what child b keeps of its parent, and its claim on the last page if
+// it is going to write there.
+__device__ void count_child(const g3k_pages_args &a, const Counts &n, int b, int lane) {
     const int cap = a.table_stride << a.page_shift;
     const int p = a.parent ? a.parent[b] : b;
     const bool real = p >= 0 && p < a.n_in;
@@ -188,15 +193,15 @@ __global__ __launch_bounds__(256) void fork_count_kernel(g3k_pages_args a) {
     for (int j = lane; j < kept; j += 64) {
         const int page = row[j];
         mine[j] = page;
-        if ((unsigned)page < (unsigned)a.num_pages) atomicAdd(&a.ref[page], 1);
+        if ((unsigned)page < (unsigned)a.num_pages) atomicAdd(&n.ref[page], 1);
     }
     if (lane) return;
     int tail = -1;
     if (want > old && (old & ((1 << a.page_shift) - 1))) {
         tail = row[old >> a.page_shift];
         if ((unsigned)tail < (unsigned)a.num_pages) {
-            atomicAdd(&a.writers[tail], 1);
-            atomicMin(&a.first[tail], b);
+            atomicAdd(&n.writers[tail], 1);
+            atomicMin(&n.first[tail], b);
         } else {
             tail = -1;      // no page to copy: the entry stays as it is
         }
@@ -212,17 +217,22 @@ __global__ __launch_bounds__(256) void fork_count_kernel(g3k_pages_args a) {
     c.copy = 0;
     a.child[b] = c;
 }
-
-__global__ __launch_bounds__(256) void compact_count_kernel(g3k_pages_args a) {
-    const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256) void fork_count_kernel(g3k_pages_args a) {
     const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= a.n_in) return;
+    if (b < a.n_out) count_child(a, {a.ref, a.writers, a.first}, b, threadIdx.x & 63);
+}
+
+__device__ void count_sequence(const g3k_pages_args &a, int *ref, int b, int lane) {
     const int n = pages_of(clampi(a.len_in[b], 0, a.table_stride << a.page_shift), a.page_shift);
     const int *row = a.table_in + (long long)b * a.table_stride;
     for (int j = lane; j < n; j += 64) {
         const int page = row[j];
-        if ((unsigned)page < (unsigned)a.num_pages) atomicAdd(&a.ref[page], 1);
+        if ((unsigned)page < (unsigned)a.num_pages) atomicAdd(&ref[page], 1);
     }
+}
+__global__ __launch_bounds__(256) void compact_count_kernel(g3k_pages_args a) {
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (b < a.n_in) count_sequence(a, a.ref, b, threadIdx.x & 63);
 }
 
 // ---- one workgroup over all pages ---------------------------------------------------
@@ -268,12 +278,11 @@ __device__ __forceinline__ int list_pages(int begin, int end, int lane, int *lis
 
 // Who copies its last page, how many pages each child needs, which children
 // get theirs, and the free pages in order.
-__global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(g3k_pages_args a) {
-    __shared__ int slot[PLAN_W];
+__device__ void plan_fork(const g3k_pages_args &a, const Counts &n, int *slot) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int begin, end, nfree, before, total;
     wave_pages(a.num_pages, wave, begin, end);
-    const int *ref = a.ref;
+    const int *ref = n.ref;
     const int mine = list_pages(begin, end, lane, nullptr, 0, 0, [ref](int p) { return ref[p] == 0; });
     const int free_before = waves_before(mine, slot, wave, lane, nfree);
     int needed = 0, given = 0, refused = 0;
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(g3k_pages_args a) {
             // the first child to write a page that all who hold it are going
             // to write keeps it; the others, and everyone where somebody
             // keeps it as it is, take a copy
-            c.copy = c.tail >= 0 && !(a.first[c.tail] == b && a.writers[c.tail] == a.ref[c.tail]);
+            c.copy = c.tail >= 0 && !(n.first[c.tail] == b && n.writers[c.tail] == n.ref[c.tail]);
             need = c.full - c.kept + c.copy;
         }
         const int upto = wave_scan_int(need);
@@ -318,12 +327,11 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(g3k_pages_args a) {
 
 // The pages in use from number `used` on, and the free ones below, in order:
 // the k-th of the one moves to the k-th of the other.
-__global__ __launch_bounds__(PLAN_T) void compact_plan_kernel(g3k_pages_args a) {
-    __shared__ int slot[PLAN_W];
+__device__ void plan_compaction(const g3k_pages_args &a, const int *ref, int *slot) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int begin, end, used, moves, holes;
     wave_pages(a.num_pages, wave, begin, end);
-    const int *ref = a.ref, *held = a.held;
+    const int *held = a.held;
     const int mine = list_pages(begin, end, lane, nullptr, 0, 0, [ref](int p) { return ref[p] != 0; });
     (void)waves_before(mine, slot, wave, lane, used);
     const auto moved = [ref, held, used](int p) { return p >= used && ref[p] != 0 && !(held && held[p]); };
@@ -343,6 +351,40 @@ __global__ __launch_bounds__(PLAN_T) void compact_plan_kernel(g3k_pages_args a) 
             a.status[1] = moves;
         }
     }
+}
+
+__global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(g3k_pages_args a) {
+    __shared__ int slot[PLAN_W];
+    plan_fork(a, {a.ref, a.writers, a.first}, slot);
+}
+__global__ __launch_bounds__(PLAN_T) void compact_plan_kernel(g3k_pages_args a) {
+    __shared__ int slot[PLAN_W];
+    plan_compaction(a, a.ref, slot);
+}
+
+// A small pool and few sequences: the counts are in LDS, and one launch takes
+// the place of three.  A wave counts two sequences at most, one after the
+// other (16 children, 2048 pages: 10.2 us against 14.3; 256 children in 1024
+// pages counted so as well, 434 against 420).
+constexpr int SMALL_PAGES = 4096, SMALL_SEQS = 2 * PLAN_W;
+__global__ __launch_bounds__(PLAN_T) void fork_small_kernel(g3k_pages_args a) {
+    __shared__ int slot[PLAN_W], ref[SMALL_PAGES], writers[SMALL_PAGES], first[SMALL_PAGES];
+    const Counts n = {ref, writers, first};
+    for (int p = threadIdx.x; p < a.num_pages; p += PLAN_T) clear_page(a, n, p);
+    __syncthreads();
+    for (int b = threadIdx.x >> 6; b < a.n_out; b += PLAN_W) count_child(a, n, b, threadIdx.x & 63);
+    __threadfence_block();
+    __syncthreads();
+    plan_fork(a, n, slot);
+}
+__global__ __launch_bounds__(PLAN_T) void compact_small_kernel(g3k_pages_args a) {
+    __shared__ int slot[PLAN_W], ref[SMALL_PAGES];
+    for (int p = threadIdx.x; p < a.num_pages; p += PLAN_T) clear_page(a, {ref, nullptr, nullptr}, p);
+    __syncthreads();
+    for (int b = threadIdx.x >> 6; b < a.n_in; b += PLAN_W) count_sequence(a, ref, b, threadIdx.x & 63);
+    __threadfence_block();
+    __syncthreads();
+    plan_compaction(a, ref, slot);
 }
 
 // ---- tables and copies ----------------------------------------------------------
@@ -421,18 +463,26 @@ extern "C" int g3k_paged_write(const g3k_paged_write_args *a, void *stream) {
 
 extern "C" int g3k_pages_fork(const g3k_pages_args *a, void *stream) {
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(pages_clear_kernel, dim3((a->num_pages + 255) / 256), dim3(256), 0, s, *a);
-    hipLaunchKernelGGL(fork_count_kernel, dim3((a->n_out + 3) / 4), dim3(256), 0, s, *a);
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    if (a->num_pages <= SMALL_PAGES && a->n_out <= SMALL_SEQS) {
+        hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    } else {
+        hipLaunchKernelGGL(pages_clear_kernel, dim3((a->num_pages + 255) / 256), dim3(256), 0, s, *a);
+        hipLaunchKernelGGL(fork_count_kernel, dim3((a->n_out + 3) / 4), dim3(256), 0, s, *a);
+        hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    }
     hipLaunchKernelGGL(fork_apply_kernel, dim3(a->n_out, a->num_layers * 2), dim3(256), 0, s, *a);
     return (int)hipGetLastError();
 }
 
 extern "C" int g3k_pages_compact(const g3k_pages_args *a, void *stream) {
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(pages_clear_kernel, dim3((a->num_pages + 255) / 256), dim3(256), 0, s, *a);
-    hipLaunchKernelGGL(compact_count_kernel, dim3((a->n_in + 3) / 4), dim3(256), 0, s, *a);
-    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    if (a->num_pages <= SMALL_PAGES && a->n_in <= SMALL_SEQS) {
+        hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    } else {
+        hipLaunchKernelGGL(pages_clear_kernel, dim3((a->num_pages + 255) / 256), dim3(256), 0, s, *a);
+        hipLaunchKernelGGL(compact_count_kernel, dim3((a->n_in + 3) / 4), dim3(256), 0, s, *a);
+        hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(PLAN_T), 0, s, *a);
+    }
     hipLaunchKernelGGL(compact_apply_kernel, dim3(a->n_in + a->copy_wgs), dim3(256), 0, s, *a);
     return (int)hipGetLastError();
 }

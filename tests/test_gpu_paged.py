@@ -130,6 +130,20 @@ def test_fork(run):
                layers=1, stride=9, label="many")
 
 
+def test_fork_and_compact_sizes(run):
+    """At and past what one launch counts by itself: 32 sequences, 4096 pages."""
+    r = run(hq=1, hkv=1)
+    rng = np.random.default_rng(8)
+    lens = [int(n) for n in rng.integers(0, 70, 20)]
+    for i, n in enumerate([31, 32, 33, 70]):
+        P.run_fork(r, lens, [int(p) for p in rng.integers(-1, 21, n)], [int(x) for x in rng.integers(-5, 30, n)], 16, 500, seed=i, stride=8,
+                   layers=1, label=f"{n} children")
+        P.run_compact(r, [int(x) for x in rng.integers(0, 70, n)], 16, 500, seed=i, layers=1, label=f"{n} sequences")
+    for i, pages in enumerate([4096, 4097]):
+        P.run_fork(r, [20, 33, 40], [0, 0, 1, 2, 2], [1, 1, 20, 1, 1], 16, pages, seed=i, layers=1, stride=5, bf16=True, label=f"{pages} pages")
+        P.run_compact(r, [20, 33, 40], 16, pages, seed=i, layers=1, bf16=True, label=f"{pages} pages")
+
+
 def test_compact(run):
     r = run(hq=2, hkv=1)
     P.run_compact(r, [20, 33, 0, 16, 1], 16, 30)

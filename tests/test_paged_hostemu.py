@@ -231,3 +231,20 @@ def test_refusals(built, tmp_path):
     r = P.EmuRunner(tmp_path, hq=4, hkv=2)
     r.lines.append("paged_refusals")
     assert "attn_emu: refused" in r.done()
+
+
+def test_fork_and_compact_sizes(built, tmp_path):
+    """At and past what one launch counts by itself: 32 sequences, 4096 pages."""
+    r = P.EmuRunner(tmp_path, hq=1, hkv=1)
+    rng = np.random.default_rng(8)
+    lens = [int(n) for n in rng.integers(0, 70, 20)]
+    for i, n in enumerate([31, 32, 33, 70]):
+        P.run_fork(r, lens, [int(p) for p in rng.integers(-1, 21, n)], [int(x) for x in rng.integers(-5, 30, n)], 16, 500, seed=i, stride=8,
+                   layers=1, label=f"{n} children")
+        P.run_compact(r, [int(x) for x in rng.integers(0, 70, n)], 16, 500, seed=i, layers=1, label=f"{n} sequences")
+    for i, pages in enumerate([4096, 4097]):
+        P.run_fork(r, [20, 33, 40], [0, 0, 1, 2, 2], [1, 1, 20, 1, 1], 16, pages, seed=i, layers=1, stride=5, bf16=True, label=f"{pages} pages")
+        P.run_compact(r, [20, 33, 40], 16, pages, seed=i, layers=1, bf16=True, label=f"{pages} pages")
+    out = r.done()
+    for kernel in ("fork_small_kernel", "fork_plan_kernel", "compact_small_kernel", "compact_plan_kernel"):
+        assert kernel in out
