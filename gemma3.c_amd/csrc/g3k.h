@@ -403,12 +403,15 @@ int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
  * Decode: group i's members [group_start[i], group_start[i + 1]) share their
  * first prefix_len[i] positions, read once per G3K_PAGED_DECODE_ROWS rows
  * through the first member's table.
- * The keys are cut into about `budget` chunks per KV head (or 2 for each run
- * of keys), at most `items` = max(budget, 2 runs) + runs, of at least min_tiles
- * 32-key tiles; runs: sequences, and for groups one each and one per
- * G3K_PAGED_DECODE_ROWS rows.  With `pack`, short sequences are one wave's
- * work.  Parts [items][n_kv_heads][part_rows]
- * rows, found through the directories dir_prefix and dir_tail [num_seqs][4]. */
+ * The keys are cut into about `budget` chunks per KV head, of at least
+ * min_tiles 32-key tiles, or more for many runs of keys; with `pack`, short
+ * sequences are one wave's work.  With runs = num_seqs + blocks, blocks =
+ * n_groups + num_seqs * group / G3K_PAGED_DECODE_ROWS (or none without groups)
+ * and extra = max(budget, min(runs, 2 budget)): items = 2 runs + extra,
+ * prefix_parts = extra + blocks, and runs more where there are at most 64
+ * sequences (none without groups).  part_rows = n_kv_heads * (prefix_parts *
+ * G3K_PAGED_DECODE_ROWS + (items + num_seqs + 8) * group) rows of parts, found
+ * through the directories dir_prefix and dir_tail [num_seqs][4]. */
 typedef struct {
     g3k_paged_seqs s;
     const void *k, *v;
@@ -421,7 +424,8 @@ typedef struct {
     float *part_o, *part_ml;   /* D floats, and (max, sum), per row */
     int n_groups;
     const int *group_start, *prefix_len;
-    int budget, min_tiles, part_rows, pack;
+    int budget, min_tiles, pack, prefix_parts;
+    long long part_rows;
     int *dir_prefix, *dir_tail;
 } g3k_paged_args;
 int g3k_paged_prefill(const g3k_paged_args *a, void *stream);

@@ -1120,8 +1120,8 @@ __device__ __forceinline__ SeqLane seq_lane(const g3k_paged_args &a, int b) {
 // there are CUs costs a second round of workgroups (8 unrelated sequences, 313
 // tiles: 36 us with 67 items a head, 21 with 64), so where the lengths are all
 // in registers the chunks are lengthened until the count fits.  Where units
-// are more than half the CUs, twice as many items as units, or the long ones
-// would hardly be cut (48 sequences in 3 groups, bf16: 77 us; 1.5 times as many
+// are more than half the CUs, twice as many items as units (two a CU more at
+// most), or the long ones would hardly be cut (48 sequences in 3 groups, bf16: 77 us; 1.5 times as many
 // 79, as many 148, 2.5 times 91).
 struct DecodePlan {
     GroupLane g0;
@@ -1152,10 +1152,11 @@ struct DecodePlan {
         alone = a.pack ? wave_sum_int(alone) : 0;
         const int packs = (alone + waves - 1) / waves;
         units = a.s.num_seqs - alone + (a.n_groups ? wave_sum_int(units) : 0);
-        const int budget = max(a.budget, (units + packs) * 2) - packs;
-        const int room = all ? budget : max(budget - units, budget / 2);
+        const int u = units + packs;
+        const int budget = max(a.budget, u + min(u, 2 * a.budget)) - packs;
+        const int room = all ? budget : budget - units;
         const float c = total * 1.0001f / (float)max(room, 1) + 1.0f;
-        per = c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
+        per = c < (float)a.min_tiles ? a.min_tiles : c < 2.f * MAX_TILES ? (int)c : 2 * MAX_TILES;
         if (!all) return;
         for (int i = 0; i < 16; i++) {
             if (wave_sum_int(g0.blocks * prefix_chunks(g0.tiles) + chunks(s0.tiles, per)) <= budget) break;
@@ -1169,10 +1170,10 @@ struct DecodePlan {
 // Or a pack: `alone`, and each wave finds its own sequence (chunks 0: none).
 struct Found {
     bool any, prefix, alone, shares;
-    int chunks, index;
+    int chunks, index, part;      // part: its number among the prefixes' chunks, or the tails', or the packs
 };
 __device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int item, int rows, int wave, int waves, int lane, Unit &u) {
-    Found r = {false, false, false, false, 0, 0};
+    Found r = {false, false, false, false, 0, 0, item};
     const auto at = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
     // the chunk's keys: its even share of the unit's tiles
     const auto keys = [&](int kbeg, int kend, int tiles) {
@@ -1217,6 +1218,7 @@ __device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int
             const int k = item - before - (at(upto, l) - at(g.blocks, l) * r.chunks);
             const int block = k / r.chunks, left = (end - first) * a.group - block * rows;
             r.any = r.prefix = true;
+            r.part = item - packs;
             r.index = k % r.chunks;
             u.b = first;
             u.run = first + block * (rows / a.group);
@@ -1566,7 +1568,6 @@ __device__ __forceinline__ void store_tail(const g3k_paged_args &a, Tail &s, cha
     }
 }
 
-// Rows of a part: a prefix chunk's ROWS, a tail chunk's group heads.
 constexpr int DECODE_WAVES = G3K_PAGED_DECODE_ROWS / 16;
 template <bool BF16>
 __global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_decode_kernel(g3k_paged_args a) {
@@ -1583,9 +1584,14 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_dec
     Unit u;
     const Found f = find_chunk(a, plan, item, ROWS, wave, NW, lane, u);
     if (!f.any) return;
-    const long long slot0 = ((long long)item * a.n_kv_heads + head) * a.part_rows;
-    // where the parts of the rows are, for the merge: item, chunks, the first
-    // one's row (a prefix's: its block's first sequence)
+    // Parts lie by what they are of, prefixes' chunks, tails' and packs: rows
+    // a part and head.  The directory has a first part's first row, the
+    // chunks, the sequence that has that row, and the rows a part.
+    const int per = f.prefix ? ROWS : f.alone ? NW * a.group : a.group;
+    if (f.prefix && f.part >= a.prefix_parts) return;      // (not so unless groups overlap)
+    const long long first0 = (f.prefix ? 0ll : (long long)a.prefix_parts * ROWS + (f.alone ? (long long)a.items * a.group : 0ll)) * a.n_kv_heads +
+                             (long long)f.part * a.n_kv_heads * per;
+    const long long slot0 = first0 + head * per;
     int *dir = (f.prefix ? a.dir_prefix : a.dir_tail) + 4 * u.run;
     if (f.alone) {
         Tail s;
@@ -1597,12 +1603,13 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, DECODE_WAVES / 4) void paged_dec
             store_tail_rows<BF16>(s, l > 0.f || l != l ? 1.0f / l : 0.f, out, lane);
             if (f.shares && lane < 16) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * (slot0 + wave * a.group + lane)) = (f32x2){s.m, l};
         }
-        if (head == 0 && lane == 0) *reinterpret_cast<u32x4 *>(dir) = (u32x4){(unsigned)item, 1, (unsigned)(wave * a.group), 0};
+        if (head == 0 && lane == 0)
+            *reinterpret_cast<u32x4 *>(dir) = (u32x4){(unsigned)first0 + wave * a.group, 1, (unsigned)u.run, (unsigned)per};
         return;
     }
     if (f.index == 0 && head == 0 && (int)threadIdx.x < (f.prefix ? u.count / a.group : 1))
         *reinterpret_cast<u32x4 *>(dir + 4 * threadIdx.x) =
-            (u32x4){(unsigned)item, (unsigned)f.chunks, f.prefix ? (unsigned)u.run : 0u, 0};
+            (u32x4){(unsigned)first0, (unsigned)f.chunks, (unsigned)u.run, (unsigned)per};
     if (!f.prefix) {
         Tail s;
         walk_tail<BF16>(a, head, u, lds, wave, NW, lane, s);
@@ -1648,16 +1655,19 @@ __global__ __launch_bounds__(256) void paged_decode_merge_kernel(g3k_paged_args 
     const int len = seq_len(a.s, b), p = seq_prefix(a, b, first);
     const bool tail = tiles_of(tail_begin(a, len, p), len) > 0;
     if (p == 0 && tail && dt.y == 1) return;        // written by its one chunk
-    const long long stride = (long long)a.n_kv_heads * a.part_rows;
     Joined j;
     j.clear();
-    const auto add = [&](u32x4 d, int row) {
-        const int item = clampi((int)d.x, 0, a.items - 1), n = clampi((int)d.y, 1, a.items - item);
-        const long long slot = ((long long)item * a.n_kv_heads + kvh) * a.part_rows + clampi(row, 0, a.part_rows - 1);
-        for (int q = 0; q < n; q += 64) j.add(a, slot + (q + min(lane, n - 1 - q)) * stride, min(n - q, 64), lane);
+    const auto add = [&](u32x4 d) {
+        const long long slot = (long long)d.x + (long long)kvh * d.w + (long long)(b - (int)d.z) * a.group + hg;
+        const long long stride = (long long)a.n_kv_heads * d.w;
+        const int n = clampi((int)d.y, 1, a.items);
+        for (int q = 0; q < n; q += 64) {
+            const long long at = slot + (q + min(lane, n - 1 - q)) * stride;
+            j.add(a, at < 0 || at >= a.part_rows ? 0 : at, min(n - q, 64), lane);
+        }
     };
-    if (tail) add(dt, (int)dt.z + hg);
-    if (p > 0) add(dp, (b - (int)dp.z) * a.group + hg);
+    if (tail) add(dt);
+    if (p > 0) add(dp);
     j.store(a.out + id * D, lane);
 }
 

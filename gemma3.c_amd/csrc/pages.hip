@@ -453,7 +453,7 @@ extern "C" int g3k_paged_write(const g3k_paged_write_args *a, void *stream) {
     const long long waves = (long long)a->s.total_q * ((nvec + WRITE_VECS - 1) / WRITE_VECS);
     if (waves <= 0) return 0;
     const long long blocks = (waves + 3) / 4;
-    if (blocks > INT_MAX) return (int)hipErrorInvalidValue;
+    if (blocks > UINT_MAX / 256) return (int)hipErrorInvalidValue;      // threads of a launch
     if (a->bf16)
         hipLaunchKernelGGL(paged_write_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a);
     else

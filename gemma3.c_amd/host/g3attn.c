@@ -2342,6 +2342,10 @@ static int bad_arg(const char *fn, const char *what) {
         if (rc_) return rc_;  \
     } while (0)
 
+static int overlap(const void *a, size_t na, const void *b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 static int aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 static int log2i(int x) {
@@ -2422,6 +2426,10 @@ int g3attn_paged_write_device(g3attn_ctx *c, int layer, const g3attn_pages *page
     if (batch->total_q == 0) return G3_OK;
     if (!Q || !K || !V || !q_out) return bad_arg(fn, "null buffer");
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(q_out)) return bad_arg(fn, "Q, K, V or q_out not 16-byte aligned");
+    const size_t nq = (size_t)batch->total_q * c->cfg.num_heads * D * sizeof(float);
+    const size_t nk = (size_t)batch->total_q * c->cfg.num_kv_heads * D * sizeof(float);
+    if ((q_out != Q && overlap(q_out, nq, Q, nq)) || overlap(q_out, nq, K, nk) || overlap(q_out, nq, V, nk))
+        return bad_arg(fn, "q_out overlaps Q without being it, or K or V");
     if (!q_norm != !k_norm) return bad_arg(fn, "one of q_norm and k_norm without the other");
     if (((uintptr_t)q_norm | (uintptr_t)k_norm) & 7) return bad_arg(fn, "norm gains not 8-byte aligned");
     g3k_paged_write_args a;
@@ -2467,8 +2475,10 @@ static void fill_paged(g3attn_ctx *c, int layer, const g3attn_pages *pages, cons
     a->out = out;
 }
 
-static int check_attention(const float *q, const float *out, const char *fn) {
+static int check_attention(const g3attn_ctx *c, const g3attn_batch *b, const float *q, const float *out, const char *fn) {
+    const size_t n = (size_t)b->total_q * c->cfg.num_heads * D * sizeof(float);
     if (!q || !out) return bad_arg(fn, "null buffer");
+    if (overlap(q, n, out, n)) return bad_arg(fn, "q and out overlap");
     if (!aligned16(q) || !aligned16(out)) return bad_arg(fn, "q or out not 16-byte aligned");
     return G3_OK;
 }
@@ -2486,7 +2496,7 @@ int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pa
     PAGED_TRY(check_pages_layer(c, layer, pages, fn));
     PAGED_TRY(check_batch(pages, batch, fn));
     if (batch->total_q == 0) return G3_OK;
-    PAGED_TRY(check_attention(q, out, fn));
+    PAGED_TRY(check_attention(c, batch, q, out, fn));
     g3k_paged_args a;
     fill_paged(c, layer, pages, batch, q, out, &a);
     const int Hkv = c->cfg.num_kv_heads;
@@ -2524,7 +2534,7 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
     PAGED_TRY(check_pages_layer(c, layer, pages, fn));
     PAGED_TRY(check_batch(pages, batch, fn));
     if (batch->q_start) return bad_arg(fn, "q_start set (one token per sequence; g3attn_paged_prefill takes more)");
-    PAGED_TRY(check_attention(q, out, fn));
+    PAGED_TRY(check_attention(c, batch, q, out, fn));
     g3k_paged_args a;
     fill_paged(c, layer, pages, batch, q, out, &a);
     const int Hkv = c->cfg.num_kv_heads, B = batch->seqs.num_seqs;
@@ -2540,13 +2550,15 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
      * of a run is a part one.  With more runs than CUs short sequences are one
      * wave's work (4 KV heads, 64 sequences behind 8192 keys; 8 heads, 48 in 3
      * groups, bf16: 55, 83 us, otherwise 106, 151). */
-    const int units = B + (a.n_groups ? a.n_groups + B * c->group / rows : 0);
+    const int blocks = a.n_groups ? a.n_groups + B * c->group / rows : 0, runs = B + blocks;
     a.budget = (c->n_cu + Hkv - 1) / Hkv;
-    a.pack = (long long)units * Hkv > c->n_cu;
-    a.items = (a.budget > 2 * units ? a.budget : 2 * units) + units;
+    a.pack = (long long)runs * Hkv > c->n_cu;
     a.min_tiles = 2;
-    a.part_rows = a.n_groups ? rows : c->group;
-    const size_t n = (size_t)a.items * Hkv * a.part_rows, ob = align256(n * D * sizeof(float)), mb = align256(n * 2 * sizeof(float));
+    const int most = runs < 2 * a.budget ? runs : 2 * a.budget, extra = a.budget > most ? a.budget : most;
+    a.items = 2 * runs + extra;
+    a.prefix_parts = a.n_groups ? extra + blocks + (B <= 64 ? runs : 0) : 0;
+    a.part_rows = Hkv * ((long long)a.prefix_parts * rows + (long long)(a.items + B + 8) * c->group);
+    const size_t n = (size_t)a.part_rows, ob = align256(n * D * sizeof(float)), mb = align256(n * 2 * sizeof(float));
     hipSetDevice(c->device);
     unsigned char *ws;
     PAGED_TRY(paged_scratch(c, ob + mb + (size_t)B * 8 * sizeof(int), fn, &ws));
@@ -2556,6 +2568,17 @@ int g3attn_paged_decode_device(g3attn_ctx *c, int layer, const g3attn_pages *pag
     a.dir_tail = a.dir_prefix + 4 * B;
     const int rc = g3k_paged_decode(&a, c->stream);
     if (rc) return hip_fail((hipError_t)rc, "g3attn_paged_decode launch");
+    return G3_OK;
+}
+
+/* Sequences may be continued in place, or in arrays of their own. */
+static int check_apart(const g3attn_seqs *from, const g3attn_seqs *to, const char *fn) {
+    const size_t row = (size_t)from->table_stride * sizeof(int);
+    if ((from->page_table != to->page_table && overlap(from->page_table, from->num_seqs * row, to->page_table, to->num_seqs * row)) ||
+        (from->kv_len != to->kv_len &&
+         overlap(from->kv_len, from->num_seqs * sizeof(int), to->kv_len, to->num_seqs * sizeof(int))) ||
+        overlap(to->kv_len, to->num_seqs * sizeof(int), to->page_table, to->num_seqs * row))
+        return bad_arg(fn, "the arrays of from and to overlap without being the same");
     return G3_OK;
 }
 
@@ -2589,6 +2612,7 @@ int g3attn_pages_fork_device(g3attn_ctx *c, const g3attn_pages *pages, const g3a
     PAGED_TRY(check_seqs(pages, from, fn));
     PAGED_TRY(check_seqs(pages, to, fn));
     if (from->table_stride != to->table_stride) return bad_arg(fn, "from and to have different table_strides");
+    PAGED_TRY(check_apart(from, to, fn));
     g3k_pages_args a;
     fill_pages(c, pages, from, to, held, status, &a);
     a.parent = parent;
@@ -2616,6 +2640,7 @@ int g3attn_pages_compact_device(g3attn_ctx *c, const g3attn_pages *pages, const 
     PAGED_TRY(check_seqs(pages, to, fn));
     if (from->table_stride != to->table_stride || from->num_seqs != to->num_seqs)
         return bad_arg(fn, "from and to have different num_seqs or table_strides");
+    PAGED_TRY(check_apart(from, to, fn));
     g3k_pages_args a;
     fill_pages(c, pages, from, to, held, status, &a);
     hipSetDevice(c->device);

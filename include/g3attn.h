@@ -419,9 +419,9 @@ typedef struct {
 
 /* The front half of a layer's attention for packed tokens: QK-norm (q_norm and
  * k_norm bf16 [256], both NULL: none) and RoPE at each token's position, with
- * the layer's table; q to q_out [total_q][num_heads * 256] (may be Q itself),
- * K (normed, rotated) and V to the token's row of its page.  Q
- * [total_q][num_heads * 256], K, V [total_q][num_kv_heads * 256], fp32.  A
+ * the layer's table; q to q_out [total_q][num_heads * 256] (Q itself, or apart
+ * from Q, K and V), K (normed, rotated) and V to the token's row of its page.
+ * Q [total_q][num_heads * 256], K, V [total_q][num_kv_heads * 256], fp32.  A
  * page that is written may not be another sequence's too
  * (g3attn_pages_fork_device sees to that).  Tokens at positions from the
  * context's max_context on, or below 0, are left out: nothing of theirs is
@@ -432,9 +432,9 @@ int g3attn_paged_write_device(g3attn_ctx *ctx, int layer, const g3attn_pages *pa
 
 /* Causal attention of packed tokens over their sequences' pages, their own
  * keys included (written before): q as g3attn_paged_write_device leaves it,
- * out [total_q][num_heads * 256].  The token at position p sees positions
- * [0, p], or [p - sliding_window + 1, p] on a local layer.  A token that sees
- * no key gets zeros; one that sees a key or value with an infinity or a NaN
+ * out [total_q][num_heads * 256], apart from q.  The token at position p sees
+ * positions [0, p], or [p - sliding_window + 1, p] on a local layer.  A token
+ * that sees no key gets zeros; one that sees a key or value with an infinity or a NaN
  * in it gives NaN, and no other one does.  Scores and products hold 22 bits of
  * q, K, V and the probabilities, with fp32 sums: about 3e-7 of the output's
  * RMS.  (The bits of a small element count from the largest magnitude among
@@ -466,15 +466,15 @@ int g3attn_paged_decode_device(g3attn_ctx *ctx, int layer, const g3attn_pages *p
  * lowest free ones, to sequences in order.  If they run out, or a table row
  * is too short, a sequence keeps its parent's length (its new positions are
  * not there).  status (may be NULL): [0] pages in use afterwards, held ones
- * included, [1] sequences that were not grown.  `to` may be `from` (same
- * arrays); both have one table_stride. */
+ * included, [1] sequences that were not grown.  `to` has from's table_stride
+ * and its arrays (each of them), or arrays apart from them. */
 int g3attn_pages_fork_device(g3attn_ctx *ctx, const g3attn_pages *pages, const g3attn_seqs *from, const int *parent,
                              const int *add, const int *held, const g3attn_seqs *to, int *status);
 
 /* Moves the pages in use to the lowest numbers, so that the rest of the pool
  * can be given up: of n pages in use, those numbered n and up move, in order,
- * into the free ones below, K and V of every layer; tables follow (`to` may be
- * `from`; same num_seqs and table_stride), entries beyond a length become -1.
+ * into the free ones below, K and V of every layer; tables follow (`to` as
+ * above, with from's num_seqs), entries beyond a length become -1.
  * Held pages (as above) count as in use and do not move.  status (may be
  * NULL): [0] pages in use, [1] pages moved. */
 int g3attn_pages_compact_device(g3attn_ctx *ctx, const g3attn_pages *pages, const g3attn_seqs *from, const int *held,

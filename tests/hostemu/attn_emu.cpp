@@ -198,10 +198,10 @@ int paged_refusals(g3attn_ctx *ctx) {
     char *const A = reinterpret_cast<char *>(1ull << 40);
     const long long rows = 2 * 16 * 256;
     const g3attn_pages pages{A, A, G3ATTN_PAGE_F32, 0, 6, 8, 16, rows, 8 * rows};
-    const g3attn_seqs seqs{2, (int *)A, (int *)A, 4};
+    const g3attn_seqs seqs{2, (int *)A, (int *)(A + (1ll << 32)), 4};
     const g3attn_batch packed{seqs, 7, (int *)A}, single{seqs, 2, nullptr};
     const float *F = (const float *)A;
-    float *O = (float *)A;
+    float *O = (float *)(A + (2ll << 32));
     const uint16_t *N = (const uint16_t *)A;
     int calls = 0;
     const auto refused = [&](int rc, const char *what) {
@@ -277,13 +277,33 @@ int paged_refusals(g3attn_ctx *ctx) {
     refused(g3attn_paged_decode_device(ctx, 0, &pages, &packed, nullptr, F, O), "decode of packed rows");
     for (int i = 0; i < 4; i++)
         for (const char *x : {(const char *)nullptr, (const char *)A + 4}) {
-            const float *a[4] = {F, F, F, F};
+            const float *a[4] = {F, F + (1 << 24), F + (2 << 24), O};
             a[i] = (const float *)x;
             refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, a[0], a[1], a[2], nullptr, nullptr, (float *)a[3]), "write buffers");
             if (i > 1) continue;
-            refused(g3attn_paged_prefill_device(ctx, 0, &pages, &packed, a[0], (float *)a[1]), "prefill buffers");
-            refused(g3attn_paged_decode_device(ctx, 0, &pages, &single, nullptr, a[0], (float *)a[1]), "decode buffers");
+            float *o = i ? (float *)x : O;
+            refused(g3attn_paged_prefill_device(ctx, 0, &pages, &packed, a[0], o), "prefill buffers");
+            refused(g3attn_paged_decode_device(ctx, 0, &pages, &single, nullptr, a[0], o), "decode buffers");
         }
+    for (long long at : {0ll, 4ll, 7 * 1024 - 4ll, -7 * 1024 + 4ll}) {
+        refused(g3attn_paged_prefill_device(ctx, 0, &pages, &packed, F, (float *)F + at), "q and out overlap");
+        if (at < 2048) refused(g3attn_paged_decode_device(ctx, 0, &pages, &single, nullptr, F, (float *)F + (at < -2044 ? -2044 : at)), "q and out overlap");
+        if (at) refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, O, O + (1 << 24), nullptr, nullptr, (float *)F + at), "Q and q_out");
+    }
+    for (int at : {0, 4, 7 * 512 - 4, -7 * 1024 + 4})
+        for (int v = 0; v < 2; v++)
+            refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, v ? F : O - at, v ? O - at : F, nullptr, nullptr, O), "q_out on K or V");
+    const g3attn_seqs far{2, seqs.kv_len + 16, seqs.page_table + 16, 4};
+    for (int i = 0; i < 5; i++) {
+        g3attn_seqs x = far;
+        if (i == 0) x.kv_len = seqs.kv_len + 1;
+        if (i == 1) x.page_table = seqs.page_table + 4;
+        if (i == 2) x.page_table = seqs.page_table - 7;
+        if (i == 3) x.kv_len = x.page_table + 7;
+        if (i == 4) x.kv_len = x.page_table - 1;
+        refused(g3attn_pages_fork_device(ctx, &pages, &seqs, nullptr, nullptr, nullptr, &x, nullptr), "arrays that overlap");
+        refused(g3attn_pages_compact_device(ctx, &pages, &seqs, nullptr, &x, nullptr), "arrays that overlap");
+    }
     refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, N, nullptr, O), "q_norm alone");
     refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, nullptr, N, O), "k_norm alone");
     refused(g3attn_paged_write_device(ctx, 0, &pages, &packed, F, F, F, N, (const uint16_t *)(A + 2), O), "k_norm alignment");

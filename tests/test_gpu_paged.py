@@ -161,7 +161,7 @@ def test_refusals(run):
     """What the host can see is refused with a message before anything is enqueued."""
     r = run(hq=4, hkv=2, layers=6)
     G, ctx = r.G, r.ctx
-    A = 1 << 40      # never followed: each call is refused first
+    A, T, O = 1 << 40, 1 << 42, 1 << 44      # never followed: each call is refused first
 
     def pages(**kw):
         d = dict(k=A, v=A, dtype=G.PAGE_F32, first_layer=0, num_layers=6, num_pages=8, page_size=16, page_stride=2 * 16 * 256,
@@ -170,7 +170,7 @@ def test_refusals(run):
         return G.Pages(**d)
 
     def seqs(**kw):
-        d = dict(num_seqs=2, kv_len=A, page_table=A, table_stride=4)
+        d = dict(num_seqs=2, kv_len=A, page_table=T, table_stride=4)
         d.update(kw)
         return G.Seqs(**d)
 
@@ -184,33 +184,33 @@ def test_refusals(run):
     for bad in (dict(k=None), dict(v=None), dict(dtype=2), dict(page_size=24), dict(page_size=8), dict(page_size=2048), dict(num_pages=0),
                 dict(num_layers=0), dict(first_layer=-1), dict(page_stride=2 * 16 * 256 - 8), dict(page_stride=2 * 16 * 256 + 4),
                 dict(layer_stride=8), dict(k=A + 4), dict(layer_stride=7 * 2 * 16 * 256)):
-        refused(ctx.paged_prefill_device, 0, pages(**bad), batch(), A, A)
+        refused(ctx.paged_prefill_device, 0, pages(**bad), batch(), A, O)
         refused(ctx.pages_compact_device, pages(**bad), seqs(), None, seqs())
     for layer, first in ((6, 0), (-1, 0), (0, 1), (5, 6)):
-        refused(ctx.paged_prefill_device, layer, pages(first_layer=first), batch(), A, A)
+        refused(ctx.paged_prefill_device, layer, pages(first_layer=first), batch(), A, O)
     for bad in (dict(num_seqs=0), dict(num_seqs=4097), dict(kv_len=None), dict(page_table=None), dict(table_stride=0), dict(table_stride=1 << 21)):
-        refused(ctx.paged_write_device, 0, pages(), batch(**bad), A, A, A, None, None, A)
-        refused(ctx.paged_decode_device, 0, pages(), batch(2, None, **bad), None, A, A)
+        refused(ctx.paged_write_device, 0, pages(), batch(**bad), A, A, A, None, None, O)
+        refused(ctx.paged_decode_device, 0, pages(), batch(2, None, **bad), None, A, O)
         refused(ctx.pages_fork_device, pages(), seqs(**bad), None, None, None, seqs())
         refused(ctx.pages_fork_device, pages(), seqs(), None, None, None, seqs(**bad))
     for b in (batch(-1), batch((1 << 24) + 1), batch(3, None), None):
-        refused(ctx.paged_prefill_device, 0, pages(), b, A, A)
-    for a in ((None, A, A, A), (A, None, A, A), (A, A, None, A), (A, A, A, None), (A + 4, A, A, A)):
+        refused(ctx.paged_prefill_device, 0, pages(), b, A, O)
+    for a in ((None, A, A, O), (A, None, A, O), (A, A, None, O), (A, A, A, None), (A + 4, A, A, O)):
         refused(ctx.paged_write_device, 0, pages(), batch(), *a[:3], None, None, a[3])
-    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A, None, A)
-    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A + 2, A, A)
-    refused(ctx.paged_prefill_device, 0, pages(), batch(), None, A)
-    refused(ctx.paged_prefill_device, 0, pages(), batch(), A, A + 8)
-    refused(ctx.paged_decode_device, 0, pages(), batch(), None, A, A)
-    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=3, group_start=A, prefix_len=A), A, A)
-    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=1, group_start=None, prefix_len=A), A, A)
-    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=-1, group_start=A, prefix_len=A), A, A)
+    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A, None, O)
+    refused(ctx.paged_write_device, 0, pages(), batch(), A, A, A, A + 2, A, O)
+    refused(ctx.paged_prefill_device, 0, pages(), batch(), None, O)
+    refused(ctx.paged_prefill_device, 0, pages(), batch(), A, O + 8)
+    refused(ctx.paged_decode_device, 0, pages(), batch(), None, A, O)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=3, group_start=A, prefix_len=A), A, O)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=1, group_start=None, prefix_len=A), A, O)
+    refused(ctx.paged_decode_device, 0, pages(), batch(2, None), G.Prefixes(num_groups=-1, group_start=A, prefix_len=A), A, O)
     refused(ctx.pages_fork_device, pages(), seqs(), None, None, None, seqs(table_stride=5))
     refused(ctx.pages_compact_device, pages(), seqs(), None, seqs(num_seqs=3))
     assert G.lib().g3attn_paged_prefill_device(None, 0, C.byref(pages()), C.byref(batch()), A, A) == G.ERR_INVALID_ARG
     ctx.paged_prefill_device(0, pages(), batch(0), None, None)      # nothing to do
     with G.Context(G.default_config(num_layers=1, max_context=16), 16, defer_rope=True) as bare:
-        refused(bare.paged_write_device, 0, pages(num_layers=1, page_stride=4 * 16 * 256), batch(), A, A, A, None, None, A)
+        refused(bare.paged_write_device, 0, pages(num_layers=1, page_stride=4 * 16 * 256), batch(), A, A, A, None, None, O)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
