@@ -14,20 +14,31 @@
 // which leaves two products.  So the matrix units do 3x (2x) the algorithmic
 // work.  Scores, maxima, sums and accumulators are fp32.
 //
-// One workgroup = 4 waves = one KV head x 64 MT query rows (a row is one
-// query head of one token; the heads of a group share the keys); each wave
-// owns 16 MT rows over the full head dim (MT blocks: Q hi / lo 64 VGPRs, O^T
-// 64 each) and walks 32-key tiles that the four waves load and convert
-// together:
+// One workgroup = 8 waves (4 for short prompts, with twice the keys a wave to
+// convert) = one KV head x 128 query rows (a row is one query
+// head of one token; the heads of a group share the keys); each wave owns 16
+// rows over the full head dim (Q hi / lo 64 VGPRs, O^T 64) and walks 32-key
+// tiles that the waves load and convert together:
 //   S^T[key][row] = K . Q^T,  O^T[dim][row] += V^T . P^T,
 // both v_mfma_f32_16x16x32_f16.  In the 16x16 accumulator lane l holds column
 // (row) l % 16, so a row's softmax state lives in the lanes l % 16 + 16 g.
+// 32 rows a wave would halve the LDS reads a row, but their O^T and Q leave no
+// registers for the tiles in flight (they spilled).
+//
+// What bounds it: packed fp32 prompts of 8192 tokens (8 heads over 4) take 441
+// us, 120 GFLOP and 378 on the matrix units, 65% of the rate a large fp16
+// product of the library reaches; matrix units busy 42% of the cycles, vector
+// units 34%, LDS 42%, at 2.0 GHz.  bf16 chunks: 285 us, 313 TFLOP/s, twice that
+// on the matrix units.  A tile takes 6400 cycles (bf16 5500): 2700 (2000) on
+// scores and values, 3300 (2900) on softmax and the next tiles' conversion, in
+// which a SIMD's two waves are opposite.  With every tile already in the cache
+// it is 3% quicker.
 //
 // LDS holds a tile as MFMA A operands in lane order (1 KiB each, so every
 // read is one conflict-free ds_read_b128): K [2 key blocks][8 dim steps], V
-// [16 dim blocks], each hi then lo.  Wave w brings keys 4w..4w+3 and
-// 16+4w..16+4w+3, one coalesced row per load.  These are the keys lane group
-// g = w of the S^T registers holds, so P goes from the S^T registers to the
+// [16 dim blocks], each hi then lo.  Wave w brings keys 16 (w / 4) + 4 g.. of
+// g = w % 4, one coalesced row per load.  These are the keys lane group g of
+// the S^T registers holds, so P goes from the S^T registers to the
 // P.V operand without a shuffle, and one scale per wave and tile is one
 // factor per lane group: K's on the scores, V's on P.  A V lane holds 4 dims
 // of the 8 keys, which are whole operand lanes of the four dim blocks
@@ -1262,6 +1273,10 @@ __device__ Found find_chunk(const g3k_paged_args &a, const DecodePlan &plan, int
 // one chunk in turn, or each all steps of a short sequence of its own.  The
 // queries' four rows lie in LDS as operand lanes, which the other 12 columns
 // of the operand read too: those columns of S^T and O^T are never used.
+// Bound by bytes: 8 unrelated sequences of 37 to 4000 keys (fp32, 4 KV heads,
+// 97 MB) take 30 us, 24 of them this kernel's: 3 to find the work, 15 for the
+// bytes, 3 to join the waves' shares; 5 the parts' merge.  As padded 128-row
+// tiles they took 62.
 template <bool BF16>
 struct Step {
     static constexpr int ROW = D * (BF16 ? 2 : 4);
