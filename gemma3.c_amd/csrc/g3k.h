@@ -394,12 +394,12 @@ int g3k_paged_write(const g3k_paged_write_args *a, void *stream);
 
 /* Attention of packed tokens (prefill) or of one token per sequence (decode)
  * over pages; q and out [total_q][heads][D].
- * Prefill: waves per workgroup, 4 or 8, 16 rows each; blocks bounds the row blocks of the batch, sum over sequences of
- * ceil(tokens * group / (16 waves)).  The keys of the longest are cut into
- * chunks of at least min_tiles 32-key tiles, to about `budget` items per KV
- * head and at most `items` (blocks + budget + 1); the parts [items][n_kv_heads]
- * [16 waves] rows are joined by a second launch.  budget 0: not cut, items =
- * blocks.
+ * Prefill: waves per workgroup, 4 or 8, 16 rows each; blocks bounds the row
+ * blocks of the batch, sum over sequences of ceil(tokens * group / (16 waves)).
+ * The keys of the longest are cut into chunks of at least min_tiles 32-key
+ * tiles, to about `budget` items per KV head or twice as many, and at most
+ * `items` (blocks + 2 budget + 1); the parts [items][n_kv_heads][16 waves] rows
+ * are joined by a second launch.  budget 0: not cut, items = blocks.
  * Decode: group i's members [group_start[i], group_start[i + 1]) share their
  * first prefix_len[i] positions, read once per G3K_PAGED_DECODE_ROWS rows
  * through the first member's table.

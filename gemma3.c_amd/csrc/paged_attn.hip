@@ -750,9 +750,10 @@ __device__ __forceinline__ Prompt prompt_of(const g3k_paged_args &a, int b, int 
 }
 
 constexpr int MAX_TILES = G3K_PAGED_MAX_LEN / BK;
+constexpr float LONG_TILES = 48.f;
 
 // Tiles per chunk: the longest blocks' keys are cut so that the batch is about
-// a.budget items per KV head, whatever the lengths.  Every wave adds the
+// a.budget items per KV head, or twice as many, whatever the lengths.  Every wave adds the
 // lengths up for itself (a causal block has keys up to its last token).
 // Without a budget nothing is cut.
 __device__ int prompt_chunk(const g3k_paged_args &a, int T, int lane) {
@@ -768,7 +769,9 @@ __device__ int prompt_chunk(const g3k_paged_args &a, int T, int lane) {
         }
         total += wave_sum(t);
     }
-    const float c = total * 1.0001f / (float)a.budget + 1.0f;
+    // (one item a CU, or two where those are long)
+    float c = total * 1.0001f / (float)a.budget + 1.0f;
+    if (c >= LONG_TILES) c = total * 1.0001f / (2.f * (float)a.budget) + 1.0f;
     return c < (float)a.min_tiles ? a.min_tiles : c < (float)MAX_TILES ? (int)c : MAX_TILES;
 }
 

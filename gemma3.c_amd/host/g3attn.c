@@ -2500,23 +2500,26 @@ int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pa
     g3k_paged_args a;
     fill_paged(c, layer, pages, batch, q, out, &a);
     const int Hkv = c->cfg.num_kv_heads;
-    /* 128 rows a workgroup read the keys half as often as 64; where they
-     * leave CUs idle, 64 are quicker (9 prompts of 1 to 120 tokens: 23 us
-     * against 27; 5 chunks behind up to 9000 cached keys, bf16: 658 against
-     * 334). */
-    a.waves = (long long)prefill_blocks(batch, c->group, 128) * Hkv < c->n_cu ? 4 : 8;
+    /* 128 rows a workgroup read the keys half as often as 64, at the same time
+     * a tile; where the prompts' own tiles (n / 64 + 1 a block at n tokens a
+     * sequence) do not fill the CUs once, 64 start sooner (9 prompts of 1 to
+     * 120 tokens: 22.5 us against 27; two prompts of 1073 tokens, bf16: 85
+     * against 68; 6 of 473, fp32: 56 against 50). */
+    const long long tiles = prefill_blocks(batch, c->group, 128) * (batch->total_q / batch->seqs.num_seqs + 64LL) / 64;
+    a.waves = tiles * Hkv < c->n_cu ? 4 : 8;
     const int rows = 16 * a.waves;
     a.blocks = a.items = prefill_blocks(batch, c->group, rows);
     hipSetDevice(c->device);
     /* Where blocks are many their different lengths even out over the CUs;
-     * else the long ones' keys are cut into two workgroups' worth a CU (fp32
-     * prompts, bf16 chunks: 456, 334 us; one a CU 443, 361; three 486, 336).
-     * Short keys are cut down to 2 tiles (the 9 short prompts: 23.1 us; down
-     * to 1, 23.6; to 4, 26). */
+     * else the long ones' keys are cut, into one workgroup's worth a CU or, if
+     * that is long, two (5 bf16 chunks, 100 tiles a CU: 286 us against 300;
+     * 4 bf16 prompts of 366 tokens, 6 a CU: 46 against 37.5).  Short keys are
+     * cut down to 2 tiles (9 short prompts: 23.1 us; down to 1, 23.6; to 4,
+     * 26). */
     if ((long long)a.blocks * Hkv <= 8LL * c->n_cu) {
-        a.budget = (2 * c->n_cu + Hkv - 1) / Hkv;
+        a.budget = (c->n_cu + Hkv - 1) / Hkv;
         a.min_tiles = 2;
-        a.items = a.blocks + a.budget + 1;
+        a.items = a.blocks + 2 * a.budget + 1;
         const size_t n = (size_t)a.items * Hkv * rows, ob = align256(n * D * sizeof(float));
         unsigned char *ws;
         PAGED_TRY(paged_scratch(c, ob + n * 2 * sizeof(float), fn, &ws));

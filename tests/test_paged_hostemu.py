@@ -248,3 +248,20 @@ def test_fork_and_compact_sizes(built, tmp_path):
     out = r.done()
     for kernel in ("fork_small_kernel", "fork_plan_kernel", "compact_small_kernel", "compact_plan_kernel"):
         assert kernel in out
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_prefill_few_cus(built, tmp_path, seed):
+    """Packed prompts of every make-up on 4 and 12 emulated CUs, where 128-row
+    workgroups run: whole and part chunks, classes, blocks that are not cut."""
+    rng = np.random.default_rng(40 + seed)
+    hq, hkv = [(2, 1), (4, 2), (4, 1), (2, 2)][seed]
+    r = P.EmuRunner(tmp_path, env={"HOSTEMU_CUS": str([4, 12][seed % 2])}, hq=hq, hkv=hkv, window=int(rng.integers(40, 200)), max_context=2048)
+    for i in range(2):
+        n = int(rng.integers(1, 6))
+        q = [int(x) for x in rng.integers(0, 120, n)]
+        hist = [int(x) for x in np.where(rng.random(n) < 0.5, 0, rng.integers(0, 500, n))]
+        P.run_prefill(r, [GLOBAL, LOCAL][i], q, [a + b for a, b in zip(q, hist)], 16, bool(rng.integers(2)), seed=seed * 10 + i,
+                      label=f"few CUs {seed}.{i}")
+    out = r.done()
+    assert "paged_prefill_merge_kernel" in out
