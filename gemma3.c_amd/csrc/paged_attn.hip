@@ -274,12 +274,13 @@ __device__ __forceinline__ float rows_max(const Raw<BF16, NW> &raw) {
     return m;
 }
 
-// The largest finite magnitude (its bits) of this wave's rows in flight, where some hold
-// an infinity or a NaN (seldom any): those rows, one bit each in `spoiled`, are
-// left out of the exponent, which is their neighbours' too.  K's become NaN,
-// and so their scores, which are masked for the rows that do not see them.
-// V's become zeros, since a value that is not finite times p = 0 is NaN in
-// every row of the product; a row that sees the key is made NaN instead.
+// The largest finite magnitude (its bits) of this wave's rows in flight, where
+// some hold an infinity or a NaN (seldom any): those rows, one bit each in
+// `spoiled`, are left out of the exponent, which is their neighbours' too.  K's
+// become NaN, and so their scores, which are masked for the rows that do not
+// see them.  V's become zeros, since a value that is not finite times p = 0 is
+// NaN in every row of the product; a row that sees the key is made NaN instead.
+// (Looking for them costs 1%.)
 template <bool KEYS, bool BF16, int NW>
 __device__ __forceinline__ int settle(Raw<BF16, NW> &raw, int &spoiled) {
     spoiled = 0;
@@ -298,9 +299,11 @@ __device__ __forceinline__ int settle(Raw<BF16, NW> &raw, int &spoiled) {
     return wave_top_bits(most);
 }
 
-// K's rows (exponent e over the wave) as operands: lane holds dims 4 lane.. = half (lane & 1) of operand
-// lane group (lane >> 1) & 3 of dim step lane >> 3.  factors[run][group]: what
-// the scores of these keys are multiplied by, and their additive mask.
+// K's rows (exponent e over the wave) as operands: lane holds dims 4 lane.. =
+// half (lane & 1) of operand lane group (lane >> 1) & 3 of dim step lane >> 3.
+// factors[run][group]: what the scores of these keys are multiplied by, and
+// their additive mask (lane 0's; the others write where nothing is read, which
+// saves a branch).
 template <bool BF16, int NW>
 __device__ __forceinline__ void store_k(const Raw<BF16, NW> &raw, int e, int bad, char *buf, f32x2 *factors, int wave, int lane) {
     using L = Lds<BF16>;
@@ -453,11 +456,8 @@ __device__ __forceinline__ void tile_scores(const char *buf, int lane, const Row
 
 // Scores to probabilities (in place), the running max and sum, and O^T's
 // rescaling, which is rare: a row's max moves only when a score outgrows it by
-// 2^LAZY.  fac[run]: the factor and mask of this lane group's keys.  other()
-// is called if `also`, in the same branch: one branch more costs 4 to 10% of
-// the whole, since nothing is scheduled across it.
-template <class Other>
-__device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, int lane, Rows &s, f32x4 (&sc)[2], bool also, Other other) {
+// 2^LAZY.  fac[run]: the factor and mask of this lane group's keys.
+__device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, int lane, Rows &s, f32x4 (&sc)[2]) {
     const int j0 = tile * BK;
     const bool ragged = j0 < s.lo_max || j0 + BK > s.hi_min;
     float t = M_NONE;
@@ -483,14 +483,13 @@ __device__ __forceinline__ void tile_softmax(const f32x2 (&fac)[2], int tile, in
         for (int r = 0; r < 4; r++) t = top(t, sc[kt][r]);
     t = col4_top(t);
     const bool up = t > s.m + LAZY;
-    if (__builtin_amdgcn_ballot_w64(up || also)) {
+    if (__builtin_amdgcn_ballot_w64(up)) {
         const float m = up ? t : s.m;
         const float keep = fast_exp2(s.m - m);
         s.m = m;
         s.l *= keep;
 #pragma unroll
         for (int d = 0; d < 16; d++) s.o[d] *= keep;
-        if (also) other();
     }
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
@@ -581,9 +580,10 @@ __device__ __forceinline__ void tile_values(const char *buf, int lane, half8 ph,
 // rows of later tiles split and stored (and the next ones fetched).  With 8
 // waves, waves w and w + 4 share a SIMD; the second four run one phase later,
 // so that one is in M while the other is in V, and store one tile further
-// ahead (`lead`).  q: this lane's row's query, if it is live.  Tile i + 2 of K goes where tile i was, i + 1 of V where i - 1
-// was, both at least a phase after their last read and before their first;
-// what V(i) needs of the factors is read in M(i), before others write them.
+// ahead (`lead`).  Tile i + 2 of K goes where tile i was, i + 1 of V where
+// i - 1 was, both at least a phase after their last read and before their
+// first; what V(i) needs of the factors is read in M(i), before others write
+// them.  q: the query of this lane's row, if it is live.
 template <bool BF16, int NW>
 __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Unit &u, char *lds, f32x2 *factors, int *exps, int wave,
                                      int lane, const float *q, bool live, Rows &s) {
@@ -652,10 +652,11 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         // (three chains of cross-lane steps side by side)
         int mk = wave_top_bits(rows_max<BF16, NW>(rk)), mv = wave_top_bits(rows_max<BF16, NW>(rv));
         spoiled = 0;
-        tile_softmax(fac, t, lane, s, p, max(mk, mv) >= NOT_FINITE, [&]() {
+        tile_softmax(fac, t, lane, s, p);
+        if (max(mk, mv) >= NOT_FINITE) {
             mk = settle<true>(rk, spoiled);
             mv = settle<false>(rv, spoiled);
-        });
+        }
         next_k(block_exponent(mk));
         next_v(block_exponent(mv), spoiled);
         G3K_WAIT_BARRIER(63);
@@ -753,9 +754,9 @@ constexpr int MAX_TILES = G3K_PAGED_MAX_LEN / BK;
 constexpr float LONG_TILES = 48.f;
 
 // Tiles per chunk: the longest blocks' keys are cut so that the batch is about
-// a.budget items per KV head, or twice as many, whatever the lengths.  Every wave adds the
-// lengths up for itself (a causal block has keys up to its last token).
-// Without a budget nothing is cut.
+// a.budget items per KV head, or twice as many, whatever the lengths.  Every
+// wave adds the lengths up for itself (a causal block has keys up to its last
+// token).  Without a budget nothing is cut.
 __device__ int prompt_chunk(const g3k_paged_args &a, int T, int lane) {
     if (a.budget <= 0) return MAX_TILES;
     float total = 0.f;      // an upper estimate
@@ -1135,8 +1136,8 @@ __device__ __forceinline__ SeqLane seq_lane(const g3k_paged_args &a, int b) {
 // tiles: 36 us with 67 items a head, 21 with 64), so where the lengths are all
 // in registers the chunks are lengthened until the count fits.  Where units
 // are more than half the CUs, twice as many items as units (two a CU more at
-// most), or the long ones would hardly be cut (48 sequences in 3 groups, bf16: 77 us; 1.5 times as many
-// 79, as many 148, 2.5 times 91).
+// most), or the long ones would hardly be cut (48 sequences in 3 groups, bf16:
+// 77 us; 1.5 times as many 79, as many 148, 2.5 times 91).
 struct DecodePlan {
     GroupLane g0;
     SeqLane s0;
