@@ -25,8 +25,8 @@
 // 32 rows a wave would halve the LDS reads a row, but their O^T and Q leave no
 // registers for the tiles in flight (they spilled).
 //
-// What bounds it: packed fp32 prompts of 8192 tokens (8 heads over 4) take 441
-// us, 120 GFLOP and 378 on the matrix units, 65% of the rate a large fp16
+// What bounds it: packed fp32 prompts of 8192 tokens (8 heads over 4) take 430
+// us, 120 GFLOP and 378 on the matrix units, 66% of the rate a large fp16
 // product of the library reaches; matrix units busy 42% of the cycles, vector
 // units 34%, LDS 42%, at 2.0 GHz.  bf16 chunks: 285 us, 313 TFLOP/s, twice that
 // on the matrix units.  A tile takes 6400 cycles (bf16 5500): 2700 (2000) on
@@ -595,12 +595,14 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
     const gbytes kb = global_bytes(a.k) + head_off, vb = global_bytes(a.v) + head_off;
     Finder<BF16, NW> find;
     // the pages, the query and the first rows are asked for before any is used
-    // (9 short prompts 22.2 us; 22.9 with the query settled first)
+    // (9 short prompts 21.7 us; 0.7 more with the query settled first)
     find.begin(a, u, lane);
     Query query;
     query.load(q, live, lane);
     Raw<BF16, NW> rk, rv;
-    int ik = 0, iv = 0;       // tiles in flight; past the end, the last one again
+    // tiles in flight; past the end nothing is fetched, and what is stored again
+    // is not read (packed fp32 8192 tokens 432 us; the last tile fetched again 446)
+    int ik = 0, iv = 0;
     auto pk = find.place(t0, wave, lane), pv = pk;
     find.fetch(kb, pk, rk);
     find.fetch(vb, pv, rv);
@@ -610,13 +612,15 @@ __device__ __forceinline__ void walk(const g3k_paged_args &a, int head, const Un
         store_k<BF16, NW>(rk, e, pk.bad, kbuf + (ik & 1) * L::K_BYTES, factors + 8 * (ik & 1), wave, lane);
         ik++;
         pv = pk;
-        pk = find.place(t0 + min(ik, n - 1), wave, lane);
-        find.fetch(kb, pk, rk);
+        if (ik < n) {
+            pk = find.place(t0 + ik, wave, lane);
+            find.fetch(kb, pk, rk);
+        }
     };
     const auto next_v = [&](int e, int spoiled) {
         store_v<BF16, NW>(rv, e, spoiled, vbuf + (iv & 1) * L::V_BYTES, exps + 8 * (iv & 1), wave, lane);
         iv++;
-        find.fetch(vb, pv, rv);
+        if (iv < n) find.fetch(vb, pv, rv);
     };
     const int lead = NW == 8 ? wave >> 2 : 0;
     int spoiled;

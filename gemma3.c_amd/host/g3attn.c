@@ -2503,7 +2503,7 @@ int g3attn_paged_prefill_device(g3attn_ctx *c, int layer, const g3attn_pages *pa
     /* 128 rows a workgroup read the keys half as often as 64, at the same time
      * a tile; where the prompts' own tiles (n / 64 + 1 a block at n tokens a
      * sequence) do not fill the CUs once, 64 start sooner (9 prompts of 1 to
-     * 120 tokens: 22.5 us against 27; two prompts of 1073 tokens, bf16: 85
+     * 120 tokens: 22 us against 27; two prompts of 1073 tokens, bf16: 85
      * against 68; 6 of 473, fp32: 56 against 50). */
     const long long tiles = prefill_blocks(batch, c->group, 128) * (batch->total_q / batch->seqs.num_seqs + 64LL) / 64;
     a.waves = tiles * Hkv < c->n_cu ? 4 : 8;
